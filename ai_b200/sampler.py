@@ -42,6 +42,58 @@ def sample_into(logits, out_ids, prm, u=None, prior=None, mask=None, B=None, ws=
               ptr(ws), 0 if ws is None else ws.numel(), stream_ptr())
 
 
+def adjust(logits, out=None, prior=None, repetition=None, presence=None, frequency=None, bias_ids=None, bias=None,
+           mask=None):
+    """Penalties, biases and grammar masks of a batch of requests, each row with its own parameters (see
+    aib_adjust_logits in include/ai_b200.h for the formula): logits [B, V] fp32 or bf16 CUDA rows -> out (default: in
+    place). repetition (> 0) / presence / frequency: fp32 [B] over the ids of prior (int32 [B, P], P <= 65535, -1 =
+    empty); bias_ids int32 / bias fp32 [B, n], n <= 1024 (biases of an id listed twice add up, ids outside the
+    vocabulary are ignored); mask int32 [B, ceil(V/32)], 1 = allowed. prior, biases and mask may be expanded from one
+    row. Returns out."""
+    if out is None:
+        out = logits
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or not logits.is_cuda:
+        raise ValueError("adjust: logits must be fp32 or bf16 CUDA rows [B, V]")
+    B, V = logits.shape
+    if B == 0 or V == 0:
+        return out
+    dev = logits.device
+    ld, out_ld = logits.stride(0), out.stride(0)
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
+        raise ValueError("adjust: out must have the shape, type and device of logits")
+    if logits.stride(1) != 1 or out.stride(1) != 1 or (B > 1 and out_ld < V):
+        raise ValueError("adjust: rows must be contiguous and the rows of out apart")
+    if out is not logits:
+        es = logits.element_size()
+        a, b = logits.data_ptr(), out.data_ptr()
+        if a < b + ((B - 1) * out_ld + V) * es and b < a + ((B - 1) * ld + V) * es and (a, ld) != (b, out_ld):
+            raise ValueError("adjust: out must be logits itself or share no memory with it")
+    args = []
+    for name, t, dtype in (("prior", prior, torch.int32), ("bias_ids", bias_ids, torch.int32),
+                           ("bias", bias, torch.float32), ("mask", mask, torch.int32)):
+        if t is None:
+            args.append((None, 0, 0))
+            continue
+        if t.dim() != 2 or t.shape[0] != B or t.dtype != dtype or t.device != dev or (t.shape[1] > 1 and
+                                                                                     t.stride(1) != 1):
+            raise ValueError(f"adjust: {name} must be {dtype} [B, n] rows on the logits' device")
+        args.append((ptr(t) if t.shape[1] else None, t.stride(0), t.shape[1]))
+    (pr, pr_ld, n_prior), (bi, bi_ld, nb), (bv, bv_ld, nv), (mk, mk_ld, nm) = args
+    if nb != nv:
+        raise ValueError("adjust: bias_ids and bias go together")
+    if mask is not None and nm != (V + 31) // 32:
+        raise ValueError("adjust: mask must have ceil(V/32) words a row")
+    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (B,) or t.device != dev or
+                              (B > 1 and t.stride(0) != 1)):
+            raise ValueError(f"adjust: {name} must be fp32 [B] on the logits' device")
+    with _lib.device_of(logits):
+        _lib.call("aib_adjust_logits", ptr(logits), ld, ptr(out), out_ld, int(logits.dtype == torch.bfloat16), B, V, pr,
+                  pr_ld, n_prior, ptr(repetition), ptr(presence), ptr(frequency), bi, bi_ld, bv, bv_ld, nb, mk, mk_ld,
+                  stream_ptr())
+    return out
+
+
 def sample(logits, temperature=0.0, top_p=1.0, top_k=0, us=None, prior=None, mask=None, repetition_penalty=1.0,
            presence_penalty=0.0, frequency_penalty=0.0, two_phase=True):
     """Convenience: returns a list of token ids. `us`: per-row uniform draws (sequence or tensor)."""

@@ -42,6 +42,7 @@ extern "C" {
 #define AIB_DEV_BAD_POS 104       /* KV position outside [0, maxt)                            */
 #define AIB_DEV_SAMPLER_CAP 105   /* sampler candidate buffer overflow                        */
 #define AIB_DEV_OVERFLOW 106      /* an output list is shorter than its CSR row pointers say  */
+#define AIB_DEV_BAD_PAGE 107      /* page id outside the pool of a paged cache                */
 
 /* One 12-bit-encoded matrix W [N, K] (K % CH == 0, CH == 256), device pointers. Same planes as the
  * reference `compress` dict (wcomp.py:13-32): m8 [N,K] = sign<<7|mantissa, e4 [N,K/2] exponent codes
@@ -224,6 +225,47 @@ int aib_attn_cached(const float* q, const uint16_t* kc, const uint16_t* vc, cons
 int aib_attn_prefill(const float* q, const uint16_t* kc, const uint16_t* vc, float* out, int n, int start, int H, int KV,
                      int HD, int maxt, float scale, void* stream);
 
+/* ------------------------------------------------------------------------------ paged cache ---- */
+/* Keys and values of many sequences in pages of one pool (no reference counterpart: its caches are contiguous,
+ * core/engine.py:234-235). k / v: bf16 bits; element d of kv head g in row r of page i is at
+ * i * page_stride + g * head_stride + r * row_stride + d (strides in elements, multiples of 8, the same for k and v;
+ * k and v 16-byte aligned). page (rows per page): a power of two. HD 64 or 128.
+ * Sequence b's row at position p is row p % page of page table[b * table_ld + p / page] (int32, p / page < max_pages).
+ * table, positions and cu are device data. A position at or past max_pages * page records AIB_DEV_BAD_POS, a page id
+ * outside [0, pages) AIB_DEV_BAD_PAGE; such rows are not written and not attended. A negative pos[b] marks an unused
+ * row of the batch. */
+typedef struct aib_paged_kv {
+  uint16_t* k;
+  uint16_t* v;
+  int64_t page_stride, head_stride, row_stride;
+  int32_t pages, page, KV, HD;
+} aib_paged_kv;
+/* Rows [T, heads, HD], elements contiguous along HD; strides in elements. */
+typedef struct aib_rows {
+  void* p;
+  int64_t token_stride, head_stride;
+} aib_rows;
+/* Appends T new tokens: k, v rows go to their pages as bf16, q rows to q_out (q, q_out: H heads, or H == 0 and NULL).
+ * Sequence b's tokens are rows cu[b] .. cu[b + 1] - 1 (int32 [B + 1], ascending), its first at position pos[b]; rows
+ * from cu[B] on, and the rows of a sequence with pos[b] < 0, are left alone. cu NULL: one token per sequence (T == B).
+ * q and k: RMSNorm over HD with weights qn / kn (bf16 [HD]; NULL: none), then the half-split rotation by
+ * position * inv[r] (fp32 [HD/2]; NULL: none), as aib_qk_rope_cache, with the angle formed in 64 bits.
+ * dtype of q, k, v, q_out: 0 fp32, 1 bf16. q_out may be q itself. No two tokens of a call may share a cache row. */
+int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
+                     const int32_t* cu, int B, int T, int H, const aib_rows* q, const aib_rows* k, const aib_rows* v,
+                     const aib_rows* q_out, int dtype, const uint16_t* qn, const uint16_t* kn, const float* inv,
+                     float eps, void* stream);
+/* Attention of one new token per sequence, its own k and v already in the cache: q [B, H, HD] (normed and rotated;
+ * rows at q_ld) attends positions max(0, pos[b] - window + 1) .. pos[b] (window 0: 0 .. pos[b]); out [B, H, HD] (rows
+ * at out_ld), lse fp32 [B, H] or NULL = log of the sum of exp(scale * q.k). A row that attends nothing gives zeros and
+ * lse -inf. dtype of q and out: 0 fp32 (products and sums as accurate as fp32), 1 bf16. H a multiple of KV.
+ * ws: aib_paged_attn_workspace(...) bytes, 16-byte aligned, zero-filled once (left zeroed where it must be); calls that
+ * may overlap on the GPU need separate ones. B <= 4096. */
+size_t aib_paged_attn_workspace(int B, int H, int KV, int HD);
+int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
+                   int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,
+                   int64_t window, float scale, void* ws, size_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------- tensor parallelism ---- */
 /* In-place sum of x (fp32 [n], n <= nmax) over the `world` tensor-parallel ranks of one node (replaces, for the
  * decode step's small blocks, the NCCL all-reduce after o_proj and down_proj; the reference has no tensor
@@ -263,6 +305,19 @@ size_t aib_sample_workspace(int B, int V);
 int aib_sample(const float* logits, int B, int V, int ld, const aib_sample_params* params, const int32_t* prior,
                int n_prior, const int32_t* bitmask, const double* u, int64_t* out_ids, void* ws, size_t ws_bytes,
                void* stream);
+/* Logit adjustment of B requests, each with its own parameters, before a sampler (no reference counterpart but the
+ * mask, generation/constrain.py:146-148). Row b of out [B, V] (row stride out_ld) from row b of logits (ld), dtype 0
+ * fp32 / 1 bf16, in fp32 and rounded once: penalties as aib_sample's over the row's prior ids (repetition over their
+ * set, then - (frequency * count + presence)); + the sum, in list order, of the row's biases of that id; -inf where the
+ * mask bit (bit j of word w = token 32w + j) is 0. repetition (> 0), presence, frequency: fp32 [B] or NULL (1, 0, 0);
+ * prior int32 [B, n_prior] (at most 65535), bias_ids int32 / bias fp32 [B, n_bias] (at most 1024): ids outside [0, V)
+ * are ignored; mask int32 [B, ceil(V/32)] or NULL. The row strides *_ld of prior, biases and mask may be 0 (one row
+ * for all). out may be logits itself (same ld), else they share no memory. */
+int aib_adjust_logits(const void* logits, int64_t ld, void* out, int64_t out_ld, int dtype, int B, int V,
+                      const int32_t* prior, int64_t prior_ld, int n_prior, const float* repetition,
+                      const float* presence, const float* frequency, const int32_t* bias_ids, int64_t bias_ids_ld,
+                      const float* bias, int64_t bias_ld, int n_bias, const int32_t* mask, int64_t mask_ld,
+                      void* stream);
 
 #ifdef __cplusplus
 }
