@@ -66,7 +66,7 @@ def test_append_refusals(L, bad):
 
 
 @pytest.mark.parametrize("bad,code", [(dict(table=None), -1), (dict(pos=None), -1), (dict(q=None), -1),
-                                      (dict(out=None), -1), (dict(B=0), -1), (dict(B=1 << 17), -1), (dict(H=3), -1),
+                                      (dict(out=None), -1), (dict(B=0), -1), (dict(B=4097), -4), (dict(H=3), -1),
                                       (dict(H=0), -1), (dict(window=-1), -1), (dict(dtype=3), -1), (dict(width=0), -1),
                                       (dict(ws=None), -3), (dict(n=1), -3)])
 def test_attention_refusals(L, bad, code):
