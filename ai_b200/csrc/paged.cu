@@ -209,15 +209,17 @@ __global__ void __launch_bounds__(32 * kAppWarps)
 // out = sum_j softmax_j(scale q.k_j) v_j in one pass over the rows with a running maximum and sum (in base 2).
 //
 // Split: the work is a line of units, a unit being 32 cached rows (from a multiple of 32) of one (sequence, key head,
-// tile of 8 query heads), and every CTA, one an SM, takes an equal run of it, so the load does not depend on how ragged
-// the lengths are and the host need not know them (a captured step keeps its grid while the sequences grow). Where a
-// (sequence, head) crosses CTAs each writes a partial state, and the last one to finish (a ticket; nobody waits) joins
-// them in order, so that the sums do not depend on timing.
+// tile of 8 query heads). Every CTA, one an SM, takes an equal run of the line and every warp an equal piece of the run,
+// so the load does not depend on how ragged the lengths are and the host need not know them (a captured step keeps its
+// grid while the sequences grow). A (sequence, head) that lies inside one warp's piece is finished there, so short
+// sequences need no joining; where it crosses warps their states are joined in shared memory at the end of the run;
+// where it crosses CTAs each writes a partial state and the last one to finish (a ticket; nobody waits) joins them. All
+// joins run in the order of the line, so the sums do not depend on timing.
 //
-// Roles in a CTA: one warp looks up pages and starts the tensor copies of K and V pages into a ring of stages; eight
-// warps take the units in turn, each with its own running state; three warps join the eight states
-// of a finished (sequence, head) and write it, while the others are already at the next one. The copies land in the
-// 128-byte swizzle, so the eight row addresses of an ldmatrix hit different banks.
+// A warp copies for itself: its lanes look up the pages of its next 32 boxes at once (a box: the rows of a page, 32 at
+// most), and one tensor copy brings a box of K or V into one of the warp's three tiles of shared memory, K of unit i + 2
+// as soon as V of unit i is used up, V of unit i + 1 when K of unit i is. The copies land in the 128-byte swizzle, so the
+// eight row addresses of an ldmatrix hit different banks. No warp waits for another before the end of its run.
 //
 // Masked rows (outside the span, or on a page outside the pool) get weight 0 and their V rows are cleared in shared
 // memory, whatever the cache holds there; boxes without a row to attend are not fetched.
@@ -228,34 +230,25 @@ __global__ void __launch_bounds__(32 * kAppWarps)
 // their weights take two parts (16 bits, 2^-8 of the output's own rounding). An mma chops its sums where an fp32 addition
 // rounds, so no long chain runs through one accumulator: the rows' running sums are added outside.
 constexpr int GT = 8;       // query heads of a group served together (the columns of an mma)
-constexpr int kCons = 8;    // warps that take units
-constexpr int kEpi = 3;     // warps that join states
-constexpr int kThreads = 32 * (1 + kEpi + kCons);
 constexpr int kBlk = 32;    // rows of a unit
-constexpr int kMinRun = 4;  // units of a CTA's run at least
+constexpr int kTiles = 3;   // tiles of a warp
 constexpr int kMaxBatch = 4096;
-constexpr int kMaxGrid = 1024;
+constexpr int kMaxGrid = 256;
 
 template <int HD>
 struct Lay {
+  static constexpr int kWarps = HD == 128 ? 8 : 12;
+  static constexpr int kThreads = 32 * kWarps;
   static constexpr int kTile = kBlk * HD * 2;           // the K or V rows of a unit: its boxes one after the other
-  static constexpr int kStages = HD == 128 ? 10 : 22;
-  static_assert(kStages >= kCons, "");
-  static constexpr int kW = HD + 2;                     // a head's sums, its maximum, its sum of weights
+  static constexpr int kRing = kWarps * kTiles * kTile;
+  static constexpr int kW = HD + 4;                     // a head's sums, its maximum, its sum of weights, padding
   static constexpr int kPart = GT * kW;                 // floats of a state
-  static constexpr int kRing = kStages * 2 * kTile;
-  static constexpr int kBytes = 1024 + kRing + kCons * kPart * 4 + kCons * GT * kBlk * 4;
+  static constexpr int kMinRun = 8;                     // units of a CTA's run at least
+  static_assert(kTiles * kTile >= kPart * 4, "a warp's last state goes where its tiles were");
+  static_assert(kWarps * kPart >= 2 * GT * kMaxGrid, "the weights of a join go where the first states were");
+  static_assert(2 * kWarps <= 32 && GT <= kWarps, "a lane for every state, a warp for every head");
 };
 
-template <int N>
-AIB_DEV void split_pair(float lo, float hi, uint32_t* w) {  // lo, hi as N bf16 parts each, (hi << 16) | lo
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    w[k] = bf16x2_rn(lo, hi);
-    lo -= __uint_as_float(w[k] << 16);
-    hi -= __uint_as_float(w[k] & 0xFFFF0000u);
-  }
-}
 // Rows [row, row + box) of head kvh in page id: [HD / 64][box][64] elements in shared memory, 128-byte swizzle.
 template <int HD>
 AIB_DEV void tma_load(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int kvh, int id) {
@@ -271,6 +264,20 @@ AIB_DEV void tma_load(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int r
         "[%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(kvh), "r"(id)
         : "memory");
+}
+template <int N>
+AIB_DEV void split_pair(float lo, float hi, uint32_t* w) {  // lo, hi as N bf16 parts each, (hi << 16) | lo
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    w[k] = bf16x2_rn(lo, hi);
+    lo -= __uint_as_float(w[k] << 16);
+    hi -= __uint_as_float(w[k] & 0xFFFF0000u);
+  }
+}
+AIB_DEV uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix of 16-bit elements, a row to four lanes
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // Rows [lo, hi) that sequence b attends; false if its position lies past the table.
@@ -316,63 +323,82 @@ AIB_DEV void seek(Cursor& c, const Line& l, int u) {  // forward to the part tha
   }
 }
 
-// Two neighbouring outputs (dimensions d, d + 1) of a head from its sums.
+AIB_DEV void add4(float4& a, float w, float4 x) {
+  a.x += w * x.x;
+  a.y += w * x.y;
+  a.z += w * x.z;
+  a.w += w * x.w;
+}
+AIB_DEV void store4(float* p, float4 a, bool vec) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = a;
+  } else {
+    p[0] = a.x, p[1] = a.y, p[2] = a.z, p[3] = a.w;
+  }
+}
+AIB_DEV void store4(uint16_t* p, float4 a, bool vec) {
+  const uint32_t lo = bf16x2_rn(a.x, a.y), hi = bf16x2_rn(a.z, a.w);
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
+  } else {
+    p[0] = lo & 0xFFFF, p[1] = lo >> 16, p[2] = hi & 0xFFFF, p[3] = hi >> 16;
+  }
+}
+AIB_DEV float lse_of(float M, float L) {
+  return M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+}
+// Four neighbouring outputs (from dimension d) of a head from its sums.
 template <typename E>
-AIB_DEV void write_out(E* out, float* lse, float M, float L, float2 a, int d) {
-  float o[2] = {M == -INFINITY ? 0.0f : a.x / L, M == -INFINITY ? 0.0f : a.y / L};
-  store_per<1>(out + d, 0, o);
-  store_per<1>(out + d + 1, 0, o + 1);
-  if (lse && d == 0) *lse = M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+AIB_DEV void write_out(E* out, float* lse, float M, float L, float4 a, int d, bool vec) {
+  const float r = M == -INFINITY ? 0.0f : 1.0f / L;
+  store4(out + d, M == -INFINITY ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(a.x * r, a.y * r, a.z * r, a.w * r),
+         vec);
+  if (lse && d == 0) *lse = lse_of(M, L);
 }
 
+struct Owner {  // what a state in shared memory belongs to (b < 0: there is none)
+  int b, s, seg0, nblk;
+};
 template <int HD>
-struct AttnShared {
-  uint64_t full_k[Lay<HD>::kStages], full_v[Lay<HD>::kStages], empty[Lay<HD>::kStages];
-  uint64_t st_full[kCons], st_free[kCons];
-  uint32_t mask[Lay<HD>::kStages];  // rows of the unit that are attended
-  long long wtot[kThreads / 32], base;
-  int b, last, fail[kEpi];
+struct Shared {
+  uint64_t full[Lay<HD>::kWarps][kTiles];
+  long long wtot[Lay<HD>::kWarps], base;
+  Owner own[2 * Lay<HD>::kWarps];  // the warps' first states (parts that began before the piece) and last states
   float M[GT], L[GT];
+  int b, abort, last[2];
 };
 
 template <int HD, typename E>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int pages, int KV,
                 int page_shift, const int32_t* __restrict__ table, int table_ld, int room,
                 const int64_t* __restrict__ pos, int B, int H, const E* __restrict__ q, long long q_ld,
                 E* __restrict__ out, long long out_ld, float* __restrict__ lse, long long window, float scale, int* cnt,
                 float* parts_ws) {
-  using L_ = Lay<HD>;
+  using Y = Lay<HD>;
   constexpr int PQ = sizeof(E) == 4 ? 3 : 1, PP = sizeof(E) == 4 ? 3 : 2;
-  constexpr int NT = HD / 16, W = L_::kW, NS = L_::kStages;
+  constexpr int NT = HD / 16, W = Y::kW, NW = Y::kWarps;
   extern __shared__ uint8_t dyn[];
-  __shared__ AttnShared<HD> sh;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* state = reinterpret_cast<float*>(ring + L_::kRing);
-  float* pws = state + kCons * L_::kPart;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* first = reinterpret_cast<float*>(ring + Y::kRing);
+  Shared<HD>& sh = *reinterpret_cast<Shared<HD>*>(first + NW * Y::kPart);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, grid = gridDim.x;
   const int G = H / KV, tiles = (G + GT - 1) / GT;
   const Line line{pos, window, B, room, KV * tiles};
-  if (threadIdx.x < NS) {
-    mbar_init(&sh.full_k[threadIdx.x], 1);
-    mbar_init(&sh.full_v[threadIdx.x], 1);
-    mbar_init(&sh.empty[threadIdx.x], 1);
-  }
-  if (threadIdx.x < kCons) {
-    mbar_init(&sh.st_full[threadIdx.x], 1);
-    mbar_init(&sh.st_free[threadIdx.x], kEpi);
-  }
-  if (warp == 0) fence_mbar_init();
+  if (lane < kTiles) mbar_init(&sh.full[warp][lane], 1);
+  if (lane < 2) sh.own[2 * warp + lane].b = -1;
   if (threadIdx.x == 0) {
+    sh.abort = 0;
     prefetch_tensormap(&kmap);
     prefetch_tensormap(&vmap);
   }
+  fence_mbar_init();
   pdl_wait();
   pdl_trigger();
 
   // ---- this CTA's run, n units from u0: a sum over the sequences' units, every thread over a few of them
-  const int cb = (B + kThreads - 1) / kThreads, b_lo = min(B, static_cast<int>(threadIdx.x) * cb),
+  const int cb = (B + Y::kThreads - 1) / Y::kThreads, b_lo = min(B, static_cast<int>(threadIdx.x) * cb),
             b_hi = min(B, b_lo + cb);
   long long mine = 0;
   for (int b = b_lo; b < b_hi; ++b) {
@@ -391,252 +417,137 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   long long total = 0, before = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < NW; ++w) {
     if (w < warp) before += sh.wtot[w];
     total += sh.wtot[w];
   }
-  const long long per = max(static_cast<long long>(kMinRun), (total + grid - 1) / grid);
+  const long long per = max(static_cast<long long>(Y::kMinRun), (total + grid - 1) / grid);
   const long long u0 = cta * per;
-  const int n = static_cast<int>(max(0LL, min(total - u0, per)));  // units of the run
+  const int n = static_cast<int>(max(0LL, min(total - u0, per)));
   if (n > 0) {
     long long base = before + incl - mine;
     if (u0 >= base && u0 < base + mine) {
       for (int b = b_lo; b < b_hi; ++b) {
         int lo, hi;
         span(pos, b, room, window, &lo, &hi);
-        const long long n = static_cast<long long>(units_of(lo, hi)) * line.parts;
-        if (u0 < base + n) {
+        const long long m = static_cast<long long>(units_of(lo, hi)) * line.parts;
+        if (u0 < base + m) {
           sh.b = b;
           sh.base = base;
           break;
         }
-        base += n;
+        base += m;
       }
     }
   }
   __syncthreads();
-  Cursor C{0, 1, 0, 0, 0, 0};
-  if (n > 0) {
+
+  // ---- the warp's piece [beg, end) of the run
+  const int piece = (n + NW - 1) / NW, beg = min(n, warp * piece), end = min(n, beg + piece);
+  const bool vec = !((reinterpret_cast<uintptr_t>(out) | out_ld * sizeof(E)) % (4 * sizeof(E)));
+  if (beg < end) {
+    Cursor C;
     C.b = sh.b;
     enter(C, line);
     C.s = static_cast<int>((u0 - sh.base) / C.nblk);
     C.seg0 = -static_cast<int>((u0 - sh.base) % C.nblk);
-  }
+    seek(C, line, beg);
 
-  if (warp <= kEpi) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == 0) {
-      // -------------------------------------------------------------------- pages -> ring of stages
-      // A lane stands for a box of rows of one page (at most 32 rows): it finds its unit, looks up its page and starts
-      // its copies, so what finding costs is shared by all the units of a batch of 32 boxes, and the next batch's
-      // look-ups run while this one's copies start.
-      const int box = min(kBlk, 1 << page_shift), nbox = kBlk / box, batch = 32 / nbox;  // units of a batch
-      const int bx = lane & (nbox - 1), bu = lane / nbox;                                // the lane's box, its unit
-      struct Look {
-        int id, row, kvh;
-        uint32_t rows;  // the box's rows that are attended, as bits of the unit
-      };
-      auto look_up = [&](int i) {
-        Look k{-1, 0, 0, 0};
-        if (i + bu < n) {
-          seek(C, line, i + bu);
-          const int j0 = (C.lo & ~(kBlk - 1)) + (i + bu - C.seg0) * kBlk, a = j0 + bx * box;
-          const int r0 = max(a, C.lo) - j0, r1 = min(a + box, C.hi) - j0;  // within the unit
-          k.kvh = C.s / tiles;
-          k.row = a & ((1 << page_shift) - 1);
-          if (r0 < r1) {
-            k.rows = (0xffffffffu >> (32 - (r1 - r0))) << r0;
-            k.id = table[static_cast<long long>(C.b) * table_ld + (a >> page_shift)];
-          }
+    // copies: a lane stands for a box of a unit
+    Cursor P = C;
+    const int box = min(kBlk, 1 << page_shift), nbox = kBlk / box, batch = 32 / nbox;  // units of a batch
+    const int bx = lane & (nbox - 1), bu = lane / nbox;                                // the lane's box, its unit
+    struct Look {
+      int id, row, kvh;
+      uint32_t rows;  // the box's rows that are attended, as bits of the unit
+    };
+    auto look_up = [&](int u) {
+      Look k{-1, 0, 0, 0};
+      if (u + bu < end) {
+        seek(P, line, u + bu);
+        const int j0 = (P.lo & ~(kBlk - 1)) + (u + bu - P.seg0) * kBlk, a = j0 + bx * box;
+        const int r0 = max(a, P.lo) - j0, r1 = min(a + box, P.hi) - j0;  // within the unit
+        k.kvh = P.s / tiles;
+        k.row = a & ((1 << page_shift) - 1);
+        if (r0 < r1) {
+          k.rows = (0xffffffffu >> (32 - (r1 - r0))) << r0;
+          k.id = table[static_cast<long long>(P.b) * table_ld + (a >> page_shift)];
         }
-        return k;
-      };
-      const uint32_t ring32 = smem_u32(ring) + bx * box * HD * 2;
-      Look next = look_up(0);
-      int st = 0, ph = 1, i = 0;
-      bool ok = true;
-      while (i < n && ok) {
-        Look k = next;
-        if (k.rows && (k.id < 0 || k.id >= pages)) {
+      }
+      return k;
+    };
+    uint8_t* my_ring = ring + warp * kTiles * Y::kTile;
+    const uint32_t tile0 = smem_u32(my_ring);
+    Look now{-1, 0, 0, 0}, next = look_up(beg);
+    uint32_t mask = 0, bytes = 0;       // of the lane's unit
+    int at = batch, iu = beg, is = 0;   // place in the batch of the unit whose copies start next, that unit, its tile
+    // starts the copies of unit iu's K (and returns the unit's attended rows) or V
+    auto start = [&](bool v) {
+      if (!v && at == batch) {
+        at = 0;
+        now = next;
+        if (now.rows && (now.id < 0 || now.id >= pages)) {
           set_status(AIB_DEV_BAD_PAGE);
-          k.rows = 0;
+          now.rows = 0;
         }
-        uint32_t mask = k.rows, bytes = k.rows ? box * HD * 2 : 0;
+        mask = now.rows;
+        bytes = now.rows ? box * HD * 2 : 0;
         for (int o = 1; o < nbox; o <<= 1) {
           mask |= __shfl_xor_sync(0xffffffffu, mask, o);
           bytes += __shfl_xor_sync(0xffffffffu, bytes, o);
         }
-        next = look_up(i + batch);
-        for (int u = 0; u < batch && i < n; ++u, ++i) {
-          ok = mbar_wait(&sh.empty[st], ph, AIB_DEV_TIMEOUT_EMPTY);
-          if (!ok) break;
-          if (lane == u * nbox) {
-            sh.mask[st] = mask;
-            mbar_arrive_expect_tx(&sh.full_k[st], bytes);
-            mbar_arrive_expect_tx(&sh.full_v[st], bytes);
-          }
-          __syncwarp();
-          if (bu == u && k.rows) {
-            const uint32_t dst = ring32 + st * 2 * L_::kTile;
-            tma_load<HD>(dst, &kmap, &sh.full_k[st], k.row, k.kvh, k.id);
-            tma_load<HD>(dst + L_::kTile, &vmap, &sh.full_v[st], k.row, k.kvh, k.id);
-          }
-          if (++st == NS) {
-            st = 0;
-            ph ^= 1;
-          }
-        }
+        next = look_up(iu + batch);
       }
-      // The consumers wait for every copy before they end. After a wait that ran out they may not, so this warp does.
-      if (!ok)
-        for (int k = 0; k < NS && --i >= 0; ++k) {
-          mbar_wait(&sh.full_k[i % NS], i / NS & 1, AIB_DEV_TIMEOUT_FULL);
-          mbar_wait(&sh.full_v[i % NS], i / NS & 1, AIB_DEV_TIMEOUT_FULL);
-        }
-    } else {
-      // ----------------------------------------------------------------- states -> outputs, partials
-      constexpr int kEt = 32 * kEpi;
-      const int et = threadIdx.x - 32, ew = warp - 1;
-      uint32_t phase = 0;
-      while (n > 0) {
-        const int beg = max(0, C.seg0), end = min(n, C.seg0 + C.nblk);
-        const int h0 = (C.s / tiles) * G + (C.s % tiles) * GT, nh = min(GT, G - (C.s % tiles) * GT);
-        const int nw = min(kCons, end - beg), w0 = beg % kCons;
-        bool ok = true;
-        for (int k = 0; k < nw; ++k) {
-          const int w = (w0 + k) % kCons;
-          ok = ok && mbar_wait(&sh.st_full[w], phase >> w & 1, AIB_DEV_TIMEOUT_FULL);
-          phase ^= 1u << w;
-        }
-        if (lane == 0) sh.fail[ew] = !ok;
-        named_sync(1, kEt);
-        bool failed = false;
-#pragma unroll
-        for (int k = 0; k < kEpi; ++k) failed = failed || sh.fail[k];
-        if (failed) break;
-        const bool whole = C.seg0 >= 0 && C.seg0 + C.nblk <= n;
-        float* part = parts_ws + static_cast<long long>(2 * cta + (C.seg0 >= 0 ? 1 : 0)) * L_::kPart;
-        E* orow = out + C.b * out_ld + static_cast<long long>(h0) * HD;
-        float* lrow = lse ? lse + static_cast<long long>(C.b) * H + h0 : nullptr;
-        for (int i = et; i < nh * (HD / 2); i += kEt) {
-          const int h = i / (HD / 2), d = i % (HD / 2) * 2;
-          float M = -INFINITY, L = 0.0f;
-          float2 a = make_float2(0.0f, 0.0f);
-          for (int k = 0; k < nw; ++k) M = fmaxf(M, state[(w0 + k) % kCons * L_::kPart + h * W + HD]);
-          const float z = M == -INFINITY ? 0.0f : M;
-          for (int k = 0; k < nw; ++k) {
-            const float* x = state + (w0 + k) % kCons * L_::kPart + h * W;
-            const float e = exp2f(x[HD] - z);
-            const float2 y = *reinterpret_cast<const float2*>(x + d);
-            L += e * x[HD + 1];
-            a.x += e * y.x;
-            a.y += e * y.y;
-          }
-          if (whole) {
-            write_out(orow + h * HD, lrow ? lrow + h : nullptr, M, L, a, d);
-          } else {
-            *reinterpret_cast<float2*>(part + h * W + d) = a;
-            if (d == 0) *reinterpret_cast<float2*>(part + h * W + HD) = make_float2(M, L);
-          }
-        }
-        __syncwarp();
-        if (lane == 0)
-          for (int k = 0; k < nw; ++k) mbar_arrive(&sh.st_free[(w0 + k) % kCons]);
-        if (!whole) {
-          // the CTAs that share this part: the last one joins their states, in order
-          const int c0 = static_cast<int>((u0 + C.seg0) / per), c1 = static_cast<int>((u0 + C.seg0 + C.nblk - 1) / per);
-          __threadfence();
-          named_sync(1, kEt);
-          if (et == 0) sh.last = atomicAdd(&cnt[c0], 1) == c1 - c0;
-          named_sync(1, kEt);
-          if (sh.last) {
-            __threadfence();
-            auto part_of = [&](int k) {  // the k-th CTA's state
-              return parts_ws + static_cast<long long>(2 * (c0 + k) + (k == 0)) * L_::kPart;
-            };
-            const int np = c1 - c0 + 1;
-            for (int h = ew; h < nh; h += kEpi) {
-              float M = -INFINITY, L = 0.0f;
-              for (int k = lane; k < np; k += 32) M = fmaxf(M, __ldcg(part_of(k) + h * W + HD));
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-              const float z = M == -INFINITY ? 0.0f : M;
-              for (int k = lane; k < np; k += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(k) + h * W + HD));
-                L += exp2f(ml.x - z) * ml.y;
-              }
-              L = warp_sum(L);
-              if (lane == 0) {
-                sh.M[h] = M;
-                sh.L[h] = L;
-              }
-            }
-            named_sync(1, kEt);
-            for (int i = et; i < nh * (HD / 2); i += kEt) {
-              const int h = i / (HD / 2), d = i % (HD / 2) * 2;
-              const float M = sh.M[h], z = M == -INFINITY ? 0.0f : M;
-              float2 a = make_float2(0.0f, 0.0f);
-#pragma unroll 8
-              for (int k = 0; k < np; ++k) {
-                const float* x = part_of(k) + h * W;
-                const float e = exp2f(__ldcg(x + HD) - z);
-                const float2 y = __ldcg(reinterpret_cast<const float2*>(x + d));
-                a.x += e * y.x;
-                a.y += e * y.y;
-              }
-              write_out(orow + h * HD, lrow ? lrow + h : nullptr, M, sh.L[h], a, d);
-            }
-            if (et == 0) cnt[c0] = 0;
-          }
-        }
-        if (end >= n) break;
-        seek(C, line, end);
+      uint64_t* bar = &sh.full[warp][is];
+      if (lane == at * nbox) mbar_arrive_expect_tx(bar, bytes);
+      __syncwarp();
+      if (bu == at && now.rows)
+        tma_load<HD>(tile0 + is * Y::kTile + bx * box * HD * 2, v ? &vmap : &kmap, bar, now.row, now.kvh, now.id);
+      const uint32_t vm = __shfl_sync(0xffffffffu, mask, at * nbox);
+      is = is == kTiles - 1 ? 0 : is + 1;
+      if (v) {
+        ++at;
+        ++iu;
       }
-      // rows of the batch that attend nothing
-      for (int b = cta; b < B; b += grid) {
-        int lo, hi;
-        span(pos, b, room, window, &lo, &hi);
-        if (hi > lo) continue;
-        const float zero = 0.0f;
-        for (int i = et; i < H * HD; i += kEt) store_per<1>(out + b * out_ld + i, 0, &zero);
-        if (lse)
-          for (int h = et; h < H; h += kEt) lse[static_cast<long long>(b) * H + h] = -INFINITY;
-      }
-    }
-    return;
-  }
+      return vm;
+    };
+    uint32_t vm = start(false), vm_next = 0;
+    start(true);
+    if (iu < end) vm_next = start(false);
 
-  // ------------------------------------------------------------------------------------ units -> states
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-  const int cw = warp - 1 - kEpi, g = lane >> 2, t = lane & 3;
-  const float sl = scale * 1.4426950408889634f;
-  float* pw = pws + cw * GT * kBlk;
-  float* mine_st = state + cw * L_::kPart;
-  const uint32_t ring32 = smem_u32(ring);
-  // ldmatrix rows: box by box, [HD / 64][box][128 bytes]. The 16-byte chunk c of the 128 bytes at address a lies in chunk
-  // c ^ (a / 128 % 8): `place` gives a with that number in the chunk's bits, to be combined with c by one xor.
-  const int box_shift = min(5, page_shift);
-  auto place = [&](int row, int half) {
-    const uint32_t a = ((row >> box_shift << box_shift) * (HD / 64) + (half << box_shift) + (row & ((1 << box_shift) - 1))) * 128;
-    return a | ((a >> 7 & 7) << 4);
-  };
-  const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kcol = lane >> 4;       // A tile of K rows: row, chunk
-  const int vr = (lane & 7) + (lane >> 4) * 8, vcol = (lane >> 3) & 1;       // V tile, transposed load
-  uint32_t ka[2][HD / 64], va[2][HD / 64];
+    // ldmatrix rows: box by box, [HD / 64][box][128 bytes]. The 16-byte chunk c of the 128 bytes at address a lies in
+    // chunk c ^ (a / 128 % 8): `place` gives a with that number in the chunk's bits, to be combined with c by one xor.
+    const int box_shift = min(5, page_shift);
+    auto place = [&](int row, int half) {
+      const uint32_t a =
+          ((row >> box_shift << box_shift) * (HD / 64) + (half << box_shift) + (row & ((1 << box_shift) - 1))) * 128;
+      return a | ((a >> 7 & 7) << 4);
+    };
+    const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kcol = lane >> 4;  // A tile of K rows: row, chunk
+    const int vr = (lane & 7) + (lane >> 4) * 8, vcol = (lane >> 3) & 1;  // V tile, transposed load
+    uint32_t ka[2][HD / 64], va[2][HD / 64];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+    for (int m = 0; m < 2; ++m)
 #pragma unroll
-    for (int h = 0; h < HD / 64; ++h) {
-      ka[m][h] = place(m * 16 + kr, h) ^ kcol << 4;
-      va[m][h] = place(m * 16 + vr, h) ^ vcol << 4;
-    }
-  uint32_t free_phase = 1;
-  int st = cw % NS, ph = 0;
-  while (n > 0) {
-    const int beg = max(0, C.seg0), end = min(n, C.seg0 + C.nblk);
-    const int h0 = (C.s / tiles) * G + (C.s % tiles) * GT, nh = min(GT, G - (C.s % tiles) * GT);
-    int u = beg + ((cw - beg) & (kCons - 1));
-    if (u < end) {
+      for (int h = 0; h < HD / 64; ++h) {
+        ka[m][h] = place(m * 16 + kr, h) ^ kcol << 4;
+        va[m][h] = place(m * 16 + vr, h) ^ vcol << 4;
+      }
+    const float sl = scale * 1.4426950408889634f;
+    int cs = 0, ph = 0, u = beg;  // tile and parity of the next wait
+    bool ok = true;
+    auto wait = [&]() {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cs], ph, AIB_DEV_TIMEOUT_FULL));
+      const int tile = cs;
+      if (++cs == kTiles) {
+        cs = 0;
+        ph ^= 1;
+      }
+      return tile;
+    };
+    while (true) {
+      const int h0 = (C.s / tiles) * G + (C.s % tiles) * GT, nh = min(GT, G - (C.s % tiles) * GT);
+      const int stop = min(end, C.seg0 + C.nblk);
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
       float acc[NT][4];
 #pragma unroll
@@ -656,14 +567,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < PQ; ++k) bq[s][k][0] = w0[k], bq[s][k][1] = w1[k];
       }
-      for (; u < end; u += kCons) {
-        const uint32_t kt = ring32 + st * 2 * L_::kTile, vt = kt + L_::kTile;
-        // A parity tells a phase from its neighbours only: this warp may be a whole round ahead of the one that has the
-        // stage's previous unit, so it waits for that one's release first. (The release before it is certain: the copying
-        // warp took it before it started this warp's last unit.)
-        if (!mbar_wait(&sh.empty[st], ph ^ 1, AIB_DEV_TIMEOUT_EMPTY)) return;
-        if (!mbar_wait(&sh.full_k[st], ph, AIB_DEV_TIMEOUT_FULL)) return;
-        const uint32_t vm = sh.mask[st];
+      for (; u < stop; ++u) {
+        const uint32_t kt = tile0 + wait() * Y::kTile;
+        if (!ok) break;
         float sc[2][4];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
@@ -680,13 +586,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[mt][i] = x[0][i] + x[1][i] + x[2][i];
         }
+        __syncwarp();
+        if (iu < end) start(true);  // V of the next unit goes where this one's K was
         // weights: sc[mt][0/1] are heads 2t, 2t+1 at row mt*16 + g, sc[mt][2/3] at row mt*16 + g + 8
         float s0[4], s1[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const bool ok = vm >> ((i >> 1) * 16 + g + (i & 1) * 8) & 1;
-          s0[i] = ok ? sc[i >> 1][(i & 1) * 2] * sl : -INFINITY;
-          s1[i] = ok ? sc[i >> 1][(i & 1) * 2 + 1] * sl : -INFINITY;
+          const bool in = vm >> ((i >> 1) * 16 + g + (i & 1) * 8) & 1;
+          s0[i] = in ? sc[i >> 1][(i & 1) * 2] * sl : -INFINITY;
+          s1[i] = in ? sc[i >> 1][(i & 1) * 2 + 1] * sl : -INFINITY;
         }
         float b0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), b1 = fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]));
 #pragma unroll
@@ -696,44 +604,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
         const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;  // no row so far: weights 0
-        float q0 = 0.0f, q1 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = (i >> 1) * 16 + g + (i & 1) * 8;
-          const float p0 = exp2f(s0[i] - z0), p1 = exp2f(s1[i] - z1);
-          q0 += p0;
-          q1 += p1;
-          pw[2 * t * kBlk + row] = p0;
-          pw[(2 * t + 1) * kBlk + row] = p1;
-        }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          q0 += __shfl_xor_sync(0xffffffffu, q0, o);
-          q1 += __shfl_xor_sync(0xffffffffu, q1, o);
-        }
         const float al0 = exp2f(m0 - z0), al1 = exp2f(m1 - z1);
-        l0 = l0 * al0 + q0;
-        l1 = l1 * al1 + q1;
         m0 = n0;
         m1 = n1;
-        __syncwarp();
-        uint32_t bp[2][PP][2];  // weights of head g at rows 16 s + 2t, +1 and +8, +9
+        l0 *= al0;
+        l1 *= al1;
+        // the weights' parts, turned from (row g, heads 2t, 2t+1) to (head g, rows 2t, 2t+1) eight rows at a time. Every
+        // lane keeps the sum over its own rows; the lanes' sums are added at the end of the part.
+        uint32_t bp[4][PP];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const float2 lo = *reinterpret_cast<const float2*>(pw + g * kBlk + s * 16 + 2 * t);
-          const float2 hi = *reinterpret_cast<const float2*>(pw + g * kBlk + s * 16 + 2 * t + 8);
-          uint32_t w0[PP], w1[PP];
-          split_pair<PP>(lo.x, lo.y, w0);
-          split_pair<PP>(hi.x, hi.y, w1);
+        for (int i = 0; i < 4; ++i) {
+          const float p0 = exp2f(s0[i] - z0), p1 = exp2f(s1[i] - z1);
+          l0 += p0;
+          l1 += p1;
+          split_pair<PP>(p0, p1, bp[i]);
 #pragma unroll
-          for (int k = 0; k < PP; ++k) bp[s][k][0] = w0[k], bp[s][k][1] = w1[k];
+          for (int k = 0; k < PP; ++k) bp[i][k] = transpose8(bp[i][k]);
         }
-        if (!mbar_wait(&sh.full_v[st], ph, AIB_DEV_TIMEOUT_FULL)) return;
-        if (vm != 0xffffffffu) {  // clear the V rows that are not attended (the copies' next write comes after this)
+        const int v_tile = wait();
+        if (!ok) break;
+        const uint32_t vt = tile0 + v_tile * Y::kTile;
+        if (vm != 0xffffffffu) {  // clear the V rows that are not attended (the tile's next copy comes after this)
           if (!(vm >> lane & 1)) {
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h) {
-              uint4* row = reinterpret_cast<uint4*>(ring + st * 2 * L_::kTile + L_::kTile + (place(lane, h) & ~127u));
+              uint4* row = reinterpret_cast<uint4*>(my_ring + v_tile * Y::kTile + (place(lane, h) & ~127u));
 #pragma unroll
               for (int c = 0; c < 8; ++c) row[c] = make_uint4(0, 0, 0, 0);
             }
@@ -749,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t a0, a1, a2, a3;
             attn::ldsm_x4_t(vt + (va[s][d / 4] ^ (d % 4 * 32)), a0, a1, a2, a3);
 #pragma unroll
-            for (int k = PP - 1; k >= 0; --k) mma_bf16(x, a0, a1, a2, a3, bp[s][k][0], bp[s][k][1]);
+            for (int k = PP - 1; k >= 0; --k) mma_bf16(x, a0, a1, a2, a3, bp[2 * s][k], bp[2 * s + 1][k]);
           }
           acc[d][0] = acc[d][0] * al0 + x[0];
           acc[d][1] = acc[d][1] * al1 + x[1];
@@ -757,33 +652,229 @@ __global__ void __launch_bounds__(kThreads, 1)
           acc[d][3] = acc[d][3] * al1 + x[3];
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.empty[st]);
-        st += kCons;
-        if (st >= NS) {
-          st -= NS;
+        vm = vm_next;
+        if (iu < end) vm_next = start(false);  // K of the unit after the next goes where this one's V was
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+      }
+      const bool began = C.seg0 >= beg, ended = C.seg0 + C.nblk <= end;
+      if (began && ended) {
+        E* o = out + C.b * out_ld + static_cast<long long>(h0) * HD + g;
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          const int h = 2 * t + hh;
+          const float M = hh ? m1 : m0, L = hh ? l1 : l0, r = M == -INFINITY ? 0.0f : 1.0f / L;
+          if (h < nh) {
+#pragma unroll
+            for (int d = 0; d < NT; ++d) {
+              const float x = M == -INFINITY ? 0.0f : acc[d][hh] * r, y = M == -INFINITY ? 0.0f : acc[d][2 + hh] * r;
+              store_per<1>(o + h * HD + d * 16, 0, &x);
+              store_per<1>(o + h * HD + d * 16 + 8, 0, &y);
+            }
+            if (lse && g == 0) lse[static_cast<long long>(C.b) * H + h0 + h] = lse_of(M, L);
+          }
+        }
+      } else {
+        float* st = ended ? first + warp * Y::kPart : reinterpret_cast<float*>(my_ring);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+          float* dst = st + (2 * t + hh) * W;
+#pragma unroll
+          for (int d = 0; d < NT; ++d) {
+            dst[d * 16 + g] = acc[d][hh];
+            dst[d * 16 + g + 8] = acc[d][2 + hh];
+          }
+          if (g == 0) {
+            dst[HD] = hh ? m1 : m0;
+            dst[HD + 1] = hh ? l1 : l0;
+          }
+        }
+        if (lane == 0) sh.own[2 * warp + (ended ? 0 : 1)] = Owner{C.b, C.s, C.seg0, C.nblk};
+      }
+      if (u >= end) break;
+      seek(C, line, u);
+    }
+    if (!ok) {  // a wait ran out: the copies that are still on their way must land before the CTA ends
+      sh.abort = 1;
+      for (int k = 0; k < kTiles; ++k) {
+        mbar_wait(&sh.full[warp][cs], ph, AIB_DEV_TIMEOUT_FULL);
+        if (++cs == kTiles) {
+          cs = 0;
           ph ^= 1;
         }
       }
-      if (!mbar_wait(&sh.st_free[cw], free_phase, AIB_DEV_TIMEOUT_EMPTY)) return;
-      free_phase ^= 1;
-#pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        float* dst = mine_st + (2 * t + hh) * W;
-#pragma unroll
-        for (int d = 0; d < NT; ++d) {
-          dst[d * 16 + g] = acc[d][hh];
-          dst[d * 16 + g + 8] = acc[d][2 + hh];
-        }
-        if (g == 0) {
-          dst[HD] = hh ? m1 : m0;
-          dst[HD + 1] = hh ? l1 : l0;
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.st_full[cw]);
     }
-    if (end >= n) break;
-    seek(C, line, end);
+  }
+  __syncthreads();
+
+  // ---- parts that cross warps: their states, neighbours among the 2 NW places, are joined in order
+  Owner o{-1, 0, 0, 0};
+  if (lane < 2 * NW) o = sh.own[lane];
+  const uint32_t there = sh.abort ? 0 : __ballot_sync(0xffffffffu, o.b >= 0);
+  if (there) {
+    const uint32_t below = there & ((1u << lane) - 1);
+    const int prev = below ? 31 - __clz(below) : 0;
+    const int pb = __shfl_sync(0xffffffffu, o.b, prev), ps = __shfl_sync(0xffffffffu, o.s, prev);
+    const uint32_t heads = __ballot_sync(0xffffffffu, o.b >= 0 && (!below || pb != o.b || ps != o.s));
+    const int ng = __popc(heads), items = min(G, GT) * (HD / 4);
+    for (int i = threadIdx.x; i < ng * items; i += Y::kThreads) {
+      uint32_t rest = heads;
+      for (int k = i / items; k > 0; --k) rest &= rest - 1;
+      const int lo = __ffs(rest) - 1;
+      rest &= rest - 1;
+      const uint32_t set = there & (0xffffffffu << lo) & (rest ? (1u << (__ffs(rest) - 1)) - 1 : 0xffffffffu);
+      const Owner w = sh.own[lo];
+      const int h = i % items / (HD / 4), d = i % (HD / 4) * 4;
+      const int h0 = (w.s / tiles) * G + (w.s % tiles) * GT;
+      if (h >= min(GT, G - (w.s % tiles) * GT)) continue;
+      auto state = [&](int k) {
+        return (k & 1 ? reinterpret_cast<const float*>(ring + (k >> 1) * kTiles * Y::kTile) : first + (k >> 1) * Y::kPart) +
+               h * W;
+      };
+      // at most one state a warp; all their loads run at once
+      float M = -INFINITY, L = 0.0f;
+      float2 ml[NW];
+      float4 y[NW];
+      uint32_t x = set;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        ml[k] = make_float2(-INFINITY, 0.0f);
+        y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (x) {
+          const float* p = state(__ffs(x) - 1);
+          ml[k] = *reinterpret_cast<const float2*>(p + HD);
+          y[k] = *reinterpret_cast<const float4*>(p + d);
+          M = fmaxf(M, ml[k].x);
+        }
+        x &= x - 1;
+      }
+      const float z = M == -INFINITY ? 0.0f : M;
+      float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float e = exp2f(ml[k].x - z);
+        add4(a, e, y[k]);
+        L += e * ml[k].y;
+      }
+      if (w.seg0 >= 0 && w.seg0 + w.nblk <= n) {
+        write_out(out + w.b * out_ld + static_cast<long long>(h0 + h) * HD,
+                  lse ? lse + static_cast<long long>(w.b) * H + h0 + h : nullptr, M, L, a, d, vec);
+      } else {
+        float* part = parts_ws + static_cast<long long>(2 * cta + (w.seg0 >= 0 ? 1 : 0)) * Y::kPart + h * W;
+        *reinterpret_cast<float4*>(part + d) = a;
+        if (d == 0) *reinterpret_cast<float2*>(part + HD) = make_float2(M, L);
+      }
+    }
+
+    // ---- parts that cross CTAs, the run's first and last at most: the last CTA to finish joins the partial states
+    const int e0 = __ffs(there) - 1, e1 = 31 - __clz(there);
+    const Owner ends[2] = {sh.own[e0], sh.own[e1]};
+    const bool one = ends[0].b == ends[1].b && ends[0].s == ends[1].s;
+    bool cross[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) cross[x] = (ends[x].seg0 < 0 || ends[x].seg0 + ends[x].nblk > n) && !(x && one);
+    if (cross[0] || cross[1]) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x < 2) {
+        const Owner w = ends[threadIdx.x];
+        bool last = false;
+        if (cross[threadIdx.x]) {
+          const int c0 = static_cast<int>((u0 + w.seg0) / per), c1 = static_cast<int>((u0 + w.seg0 + w.nblk - 1) / per);
+          last = atomicAdd(&cnt[c0], 1) == c1 - c0;
+          if (last) {
+            cnt[c0] = 0;
+            __threadfence();
+          }
+        }
+        sh.last[threadIdx.x] = last;
+      }
+      __syncthreads();
+      // A thread has four dimensions of a head and every other state, so that all its loads run at once.
+      float* pm = first;                  // [GT][kMaxGrid]: the states' maxima, then their weights
+      float* pl = pm + GT * kMaxGrid;     // their sums
+      for (int x = 0; x < 2; ++x) {
+        if (!sh.last[x]) continue;
+        const Owner w = ends[x];
+        const int c0 = static_cast<int>((u0 + w.seg0) / per), np = static_cast<int>((u0 + w.seg0 + w.nblk - 1) / per) - c0 + 1;
+        const int h0 = (w.s / tiles) * G + (w.s % tiles) * GT, nh = min(GT, G - (w.s % tiles) * GT);
+        auto part_of = [&](int k) {  // the k-th CTA's state
+          return parts_ws + static_cast<long long>(2 * (c0 + k) + (k == 0)) * Y::kPart;
+        };
+        for (int i = threadIdx.x; i < nh * np; i += Y::kThreads) {
+          const int h = i % nh, k = i / nh;
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(k) + h * W + HD));
+          pm[h * kMaxGrid + k] = ml.x;
+          pl[h * kMaxGrid + k] = ml.y;
+        }
+        auto weigh = [&]() {  // a warp for every head; all threads come here once
+          __syncthreads();
+          if (warp < nh) {
+            float* m = pm + warp * kMaxGrid;
+            float M = -INFINITY, L = 0.0f;
+            for (int k = lane; k < np; k += 32) M = fmaxf(M, m[k]);
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+            const float z = M == -INFINITY ? 0.0f : M;
+            for (int k = lane; k < np; k += 32) {
+              const float e = exp2f(m[k] - z);
+              m[k] = e;
+              L += e * pl[warp * kMaxGrid + k];
+            }
+            L = warp_sum(L);
+            if (lane == 0) {
+              sh.M[warp] = M;
+              sh.L[warp] = L;
+            }
+          }
+          __syncthreads();
+        };
+        constexpr int kDeep = 8;
+        const int half = lane >> 4;
+        bool weighed = false;
+        for (int i = warp * 16 + (lane & 15); i < nh * (HD / 4); i += Y::kThreads / 2) {  // whole warps go round
+          const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+          float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int k0 = half; k0 < np + half; k0 += 2 * kDeep) {
+            float4 y[kDeep];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+              y[k] = __ldcg(reinterpret_cast<const float4*>(part_of(min(k0 + 2 * k, np - 1)) + h * W + d));
+            if (!weighed) {
+              weigh();
+              weighed = true;
+            }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+              if (k0 + 2 * k < np) add4(a, pm[h * kMaxGrid + k0 + 2 * k], y[k]);
+          }
+          a.x += __shfl_xor_sync(0xffffffffu, a.x, 16);
+          a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+          a.z += __shfl_xor_sync(0xffffffffu, a.z, 16);
+          a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+          if (half == 0)
+            write_out(out + w.b * out_ld + static_cast<long long>(h0 + h) * HD,
+                      lse ? lse + static_cast<long long>(w.b) * H + h0 + h : nullptr, sh.M[h], sh.L[h], a, d, vec);
+        }
+        if (!weighed) weigh();
+        __syncthreads();  // the weights are rewritten next
+      }
+    }
+  }
+
+  // ---- rows of the batch that attend nothing
+  for (int b = cta; b < B; b += grid) {
+    int lo, hi;
+    span(pos, b, room, window, &lo, &hi);
+    if (hi > lo) continue;
+    const float zero = 0.0f;
+    for (int i = threadIdx.x; i < H * HD; i += Y::kThreads) store_per<1>(out + b * out_ld + i, 0, &zero);
+    if (lse)
+      for (int h = threadIdx.x; h < H; h += Y::kThreads) lse[static_cast<long long>(b) * H + h] = -INFINITY;
   }
 }
 
@@ -832,6 +923,11 @@ static size_t attn_ws_bytes(int HD) {
          static_cast<size_t>(2) * max_grid() * (HD == 128 ? Lay<128>::kPart : Lay<64>::kPart) * sizeof(float);
 }
 
+template <int HD>
+static constexpr size_t smem_bytes() {
+  return 1024 + Lay<HD>::kRing + Lay<HD>::kWarps * Lay<HD>::kPart * sizeof(float) + sizeof(Shared<HD>);
+}
+
 // Tensor map of the pool: boxes of HD elements (in halves of 128 bytes, swizzled) x the rows of a page, 32 at most.
 static int pool_map(CUtensorMap* map, const uint16_t* p, const aib_paged_kv* c) {
   const uint64_t HD = c->HD, halves = HD / 64, page = c->page, KV = c->KV, pages = c->pages;
@@ -854,7 +950,7 @@ static int attend(const aib_paged_kv* c, const int32_t* table, int table_ld, int
                   const void* q, long long q_ld, void* out, long long out_ld, float* lse, long long window, float scale,
                   void* ws, cudaStream_t s) {
   const int G = H / c->KV, tiles = (G + GT - 1) / GT;
-  int rc = allow_smem(attn_kernel<HD, E>, Lay<HD>::kBytes);
+  int rc = allow_smem(attn_kernel<HD, E>, smem_bytes<HD>());
   CUtensorMap kmap, vmap;
   if (!rc) rc = pool_map(&kmap, c->k, c);
   if (!rc) rc = pool_map(&vmap, c->v, c);
@@ -862,8 +958,8 @@ static int attend(const aib_paged_kv* c, const int32_t* table, int table_ld, int
   // no more CTAs than the longest sequences the table allows could fill
   const long long rows = window > 0 ? std::min<long long>(window + kBlk - 1, room) : room;
   const long long units = static_cast<long long>(B) * c->KV * tiles * ((rows + kBlk - 1) / kBlk);
-  const int grid = static_cast<int>(std::min<long long>(max_grid(), (units + kMinRun - 1) / kMinRun));
-  return launch(attn_kernel<HD, E>, dim3(grid), dim3(kThreads), Lay<HD>::kBytes, s, "aib_paged_attn", kmap, vmap,
+  const int grid = static_cast<int>(std::min<long long>(max_grid(), (units + Lay<HD>::kMinRun - 1) / Lay<HD>::kMinRun));
+  return launch(attn_kernel<HD, E>, dim3(grid), dim3(Lay<HD>::kThreads), smem_bytes<HD>(), s, "aib_paged_attn", kmap, vmap,
                 c->pages, c->KV, __builtin_ctz(c->page), table, table_ld, room, pos, B, H, static_cast<const E*>(q),
                 q_ld, static_cast<E*>(out), out_ld, lse, window, scale, static_cast<int*>(ws),
                 reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kMaxGrid * sizeof(int)));
