@@ -6,6 +6,8 @@ become exceptions (ValueError for bad arguments, like the reference launchers, R
 import ctypes as C
 import os
 
+import torch
+
 from . import build as _build
 
 LIB_PATH = _build.LIB
@@ -32,11 +34,6 @@ class PagedKv(C.Structure):
     """Mirror of `aib_paged_kv`."""
     _fields_ = [("k", P), ("v", P), ("page_stride", I64), ("head_stride", I64), ("row_stride", I64), ("pages", I32),
                 ("page", I32), ("KV", I32), ("HD", I32)]
-
-
-class Rows(C.Structure):
-    """Mirror of `aib_rows`."""
-    _fields_ = [("p", P), ("token_stride", I64), ("head_stride", I64)]
 
 
 # name -> (restype, argtypes); every function declared in include/ai_b200.h
@@ -76,10 +73,10 @@ SIGNATURES = {
     "aib_qk_rope_cache": (I32, [P, P, P, P, P, P, P, P, I32, I32, I32, I32, I32, F32, P]),
     "aib_attn_cached": (I32, [P, P, P, P, P, I32, I32, I32, I32, I32, F32, P, SZ, P]),
     "aib_attn_prefill": (I32, [P, P, P, P, I32, I32, I32, I32, I32, I32, F32, P]),
-    "aib_paged_append": (I32, [C.POINTER(PagedKv), P, I32, I32, P, P, I32, I32, I32, C.POINTER(Rows), C.POINTER(Rows),
-                               C.POINTER(Rows), C.POINTER(Rows), I32, P, P, P, F32, P]),
+    "aib_paged_append": (I32, [C.POINTER(PagedKv), P, I64, I32, P, P, I32, I32, I32, P, I64, I64, P, I64, I64, P, I64,
+                               I64, P, I64, I64, I32, P, P, P, F32, P]),
     "aib_paged_attn_workspace": (SZ, [I32, I32, I32, I32]),
-    "aib_paged_attn": (I32, [C.POINTER(PagedKv), P, I32, I32, P, I32, I32, P, I64, P, I64, I32, P, I64, F32, P, SZ, P]),
+    "aib_paged_attn": (I32, [C.POINTER(PagedKv), P, I64, I32, P, I32, I32, P, I64, P, I64, I32, P, I64, F32, P, SZ, P]),
     "aib_adjust_logits": (I32, [P, I64, P, I64, I32, I32, I32, P, I64, I32, P, P, P, P, I64, P, I64, I32, P, I64, P]),
     "aib_sample_workspace": (SZ, [I32, I32]),
     "aib_sample": (I32, [P, I32, I32, I32, C.POINTER(SampleParams), P, I32, P, P, P, P, SZ, P]),
@@ -132,26 +129,27 @@ def ptr(t):
 
 
 def stream_ptr(stream=None):
-    import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return C.c_void_p(s.cuda_stream)
+    """A stream's handle; without one, that of the current device's current stream."""
+    if stream is not None:
+        return C.c_void_p(stream.cuda_stream)
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
-class device_of:
-    """Makes a tensor's device current for a call (a launch goes to the current device's stream)."""
+class on_device:
+    """Makes device `index` current for a call (a launch goes to the current device) and gives its current stream's
+    handle."""
     __slots__ = ("new", "old")
 
-    def __init__(self, t):
-        self.new = t.device.index
+    def __init__(self, index):
+        self.new = index
 
     def __enter__(self):
-        import torch
         self.old = torch.cuda.current_device()
         if self.old != self.new:
             torch.cuda.set_device(self.new)
+        return torch._C._cuda_getCurrentRawStream(self.new)
 
     def __exit__(self, *exc):
         if self.old != self.new:
-            import torch
             torch.cuda.set_device(self.old)
         return False

@@ -6,6 +6,7 @@
 // checked where it is used: a position past the table's last page records AIB_DEV_BAD_POS, a page id outside the pool
 // AIB_DEV_BAD_PAGE, and the row is neither written nor attended.
 #include <algorithm>
+#include <atomic>
 #include "common.cuh"
 
 namespace aib {
@@ -18,55 +19,55 @@ struct Kv {
   int pages, KV;
   int page_shift;  // rows per page = 1 << page_shift
 };
-// [T, heads, HD] rows: token and head strides in elements, inner stride 1; vec: pairs may be read as one word
+// [T, heads, HD] rows: token and head strides in elements, inner stride 1
 template <typename E>
 struct Rows {
   E* p;
   long long ts, hs;
-  int vec;
 };
 
-// A pair of neighbouring elements (HD 128) or one element (HD 64) per lane as floats, and back.
-template <int PER>
-AIB_DEV void load_per(const float* p, int vec, float* o) {
-  if (PER == 2 && vec) {
-    const float2 t = *reinterpret_cast<const float2*>(p);
-    o[0] = t.x;
-    o[1] = t.y;
+// Four neighbouring elements as floats and back; VEC: in one access (16 bytes of fp32, 8 of bf16), evicted first since they
+// are read once (16384 prompt tokens: 135 us with plain loads, 119 us with these).
+template <bool VEC>
+AIB_DEV void load4(const float* p, float* o) {
+  if (VEC) {
+    const float4 t = __ldcs(reinterpret_cast<const float4*>(p));
+    o[0] = t.x, o[1] = t.y, o[2] = t.z, o[3] = t.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = p[i];
+    for (int i = 0; i < 4; ++i) o[i] = p[i];
   }
 }
-template <int PER>
-AIB_DEV void load_per(const uint16_t* p, int vec, float* o) {
-  if (PER == 2 && vec) {
-    const uint32_t t = *reinterpret_cast<const uint32_t*>(p);
-    o[0] = __uint_as_float(t << 16);
-    o[1] = __uint_as_float(t & 0xFFFF0000u);
+template <bool VEC>
+AIB_DEV void load4(const uint16_t* p, float* o) {
+  if (VEC) {
+    const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
+    o[0] = __uint_as_float(t.x << 16), o[1] = __uint_as_float(t.x & 0xFFFF0000u);
+    o[2] = __uint_as_float(t.y << 16), o[3] = __uint_as_float(t.y & 0xFFFF0000u);
   } else {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) o[i] = bf16_to_f32(p[i]);
+    for (int i = 0; i < 4; ++i) o[i] = bf16_to_f32(p[i]);
   }
 }
-template <int PER>
-AIB_DEV void store_per(float* p, int vec, const float* o) {
-  if (PER == 2 && vec) {
-    *reinterpret_cast<float2*>(p) = make_float2(o[0], o[PER - 1]);
+AIB_DEV void store4(float* p, float4 a, bool vec) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = a;
   } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) p[i] = o[i];
+    p[0] = a.x, p[1] = a.y, p[2] = a.z, p[3] = a.w;
   }
 }
-template <int PER>
-AIB_DEV void store_per(uint16_t* p, int vec, const float* o) {
-  if (PER == 2 && vec) {
-    *reinterpret_cast<uint32_t*>(p) = bf16x2_rn(o[0], o[PER - 1]);
+AIB_DEV void store4(uint16_t* p, float4 a, bool vec) {
+  const uint32_t lo = bf16x2_rn(a.x, a.y), hi = bf16x2_rn(a.z, a.w);
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
   } else {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) p[i] = bf16_rn(o[i]);
+    p[0] = lo & 0xFFFF, p[1] = lo >> 16, p[2] = hi & 0xFFFF, p[3] = hi >> 16;
   }
 }
+AIB_DEV float to_f32(float x) { return x; }
+AIB_DEV float to_f32(uint16_t x) { return bf16_to_f32(x); }
+AIB_DEV void from_f32(float x, float* o) { *o = x; }
+AIB_DEV void from_f32(float x, uint16_t* o) { *o = bf16_rn(x); }
 
 // cos and sin of p * inv. The product is formed in 64 bits (exact: 31 x 24 bits fit with at most one rounding in the
 // last place) and reduced by whole turns there, so a far position loses nothing; a float product would be off by
@@ -78,130 +79,177 @@ AIB_DEV void rotation(long long p, float inv, float* c, float* s) {
   sincosf(r, s, c);
 }
 
-// Largest b in [0, B) with cu[b] <= t (0 if none): the warp probes 32 places a round. cu is device data: whatever it
-// holds, the result is in range.
-AIB_DEV int find_seq(const int32_t* cu, int B, int t) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = B;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int i = lo + lane * step;
-    const unsigned m = __ballot_sync(0xffffffffu, i < hi && cu[i] <= t);
-    const int n = max(1, __popc(m));
+// The sequence of token t (cu NULL: one token each) and its position: b, the position's first token's, the offset.
+// Sequences are found 32 places a round, with the positions of the places probed read along with them. cu is device
+// data: whatever it holds, b is in range. False for a row behind the last sequence.
+AIB_DEV bool find_seq(const int32_t* cu, const int64_t* pos, int B, int t, int* b, long long* p0, int* off) {
+  if (!cu) {
+    *b = t;
+    *p0 = pos[t];
+    *off = 0;
+    return true;
+  }
+  const int lane = threadIdx.x & 31, total = cu[B];
+  int lo = 0, hi = B, c = 0;
+  long long p = 0;
+  while (true) {
+    const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+    if (i < hi) {
+      c = cu[i];
+      p = pos[i];
+    }
+    const int n = max(1, __popc(__ballot_sync(0xffffffffu, i < hi && c <= t)));
     lo += (n - 1) * step;
     hi = min(hi, lo + step);
+    if (step == 1 || hi - lo == 1) {
+      *b = lo;
+      *off = t - __shfl_sync(0xffffffffu, c, n - 1);
+      *p0 = __shfl_sync(0xffffffffu, p, n - 1);
+      return t < total && *off >= 0;
+    }
   }
-  return lo;
 }
 
+// One warp takes `per` of a token's head vectors (q heads, then k heads, then v heads), several at a time: a vector has
+// LPV lanes, a lane four dimensions from r on and their rotation partners HD/2 further, so a vector is read and written
+// with 16-byte accesses and norm and rotation need no exchange but the sum of squares. The norm's weights are folded
+// into the token's cosines and sines, which a warp computes once. The first vectors are on their way before the warp
+// looks for its sequence, position and page, the next ones while it works.
+// Bound by bytes for prompts (issue slots come next: 25 instructions a vector of 128), by latency for single tokens.
 constexpr int kAppWarps = 8;
-constexpr int kAppBatch = 4;  // head vectors a warp holds at once
+constexpr int kAppSteps = 2;  // steps of 32 / LPV vectors in hand, and as many on their way
 
-// One warp takes `per` of a token's head vectors (q heads, then k heads, then v heads); the lane holds dimensions
-// r .. r + PER - 1 and their rotation partners HD/2 further, so norm and rotation need no exchange but the sum of
-// squares, and the token's cosines and sines are computed once per warp.
-template <int HD, typename E>
+template <int HD, typename E, bool VEC>
 __global__ void __launch_bounds__(32 * kAppWarps)
-    append_kernel(Kv c, const int32_t* __restrict__ table, int table_ld, int max_pages, const int64_t* __restrict__ pos,
-                  const int32_t* __restrict__ cu, int B, int T, int H, Rows<const E> q, Rows<const E> k,
-                  Rows<const E> v, Rows<E> qo, const uint16_t* __restrict__ qn, const uint16_t* __restrict__ kn,
-                  const float* __restrict__ inv, float eps, int parts, int per) {
-  constexpr int PER = HD / 64, HALF = HD / 2;
+    append_kernel(Kv c, const int32_t* __restrict__ table, long long table_ld, int max_pages,
+                  const int64_t* __restrict__ pos, const int32_t* __restrict__ cu, int B, int T, int H, Rows<const E> q,
+                  Rows<const E> k, Rows<const E> v, Rows<E> qo, const uint16_t* __restrict__ qn,
+                  const uint16_t* __restrict__ kn, const float* __restrict__ inv, float eps, int parts, int per) {
+  constexpr int LPV = HD / 8, VPW = 32 / LPV, HALF = HD / 2, BATCH = kAppSteps * VPW;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * kAppWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, sub = lane / LPV, r = lane % LPV * 4;
+  const unsigned w = blockIdx.x * kAppWarps + (threadIdx.x >> 5);
   const int t = static_cast<int>(w / parts);
   if (t >= T) return;
-  int b = t, off = 0;
-  if (cu) {
-    if (t >= cu[B]) return;  // a row behind the last sequence
-    b = find_seq(cu, B, t);
-    off = t - cu[b];
-    if (off < 0) return;
-  }
-  const long long p0 = pos[b], p = p0 + off;
-  if (p0 < 0) return;  // an unused row of the batch
-  const int r = lane * PER;
-  float cs[PER], sn[PER];
+  const int KV = c.KV, nv = H + 2 * KV, v0 = static_cast<int>(w % parts) * per, v1 = min(nv, v0 + per);
+  // a batch has vectors of one kind: [h0, stop)
+  auto stop_of = [&](int h0) { return min(min(h0 + BATCH, v1), h0 < H ? H : (h0 < H + KV ? H + KV : nv)); };
+  auto load = [&](int h0, float (*x)[8]) {
+    if (h0 >= v1) return;
+    const Rows<const E> src = h0 < H ? q : (h0 < H + KV ? k : v);
+    const int first = h0 < H ? 0 : (h0 < H + KV ? H : H + KV), stop = stop_of(h0);
+    const E* p = src.p + t * src.ts + (h0 - first + sub) * src.hs + r;
+#pragma unroll
+    for (int i = 0; i < kAppSteps; ++i) {
+      if (h0 + sub + i * VPW < stop) {
+        load4<VEC>(p, x[i]);
+        load4<VEC>(p + HALF, x[i] + 4);
+      }
+      p += VPW * src.hs;
+    }
+  };
+  float x[kAppSteps][8];
+  load(v0, x);
+  float f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (inv) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) rotation(p, inv[r + i], &cs[i], &sn[i]);
+    for (int i = 0; i < 4; ++i) f[i] = inv[r + i];
   }
+  int b, off;
+  long long p0;
+  if (!find_seq(cu, pos, B, t, &b, &p0, &off) || p0 < 0) return;  // behind the last sequence, or an unused row
+  const long long p = p0 + off;
   // where the token's k and v rows go
-  const long long pg = p >> c.page_shift;
   long long row = -1;
-  if (pg >= max_pages) {
-    if (lane == 0) set_status(AIB_DEV_BAD_POS);
-  } else {
-    const int id = table[static_cast<long long>(b) * table_ld + pg];
-    if (id < 0 || id >= c.pages) {
-      if (lane == 0) set_status(AIB_DEV_BAD_PAGE);
+  if (v1 > H) {
+    const long long pg = p >> c.page_shift;
+    if (pg >= max_pages) {
+      if (lane == 0) set_status(AIB_DEV_BAD_POS);
     } else {
-      row = id * c.page_stride + (p & ((1 << c.page_shift) - 1)) * c.row_stride;
+      const int id = table[b * table_ld + pg];
+      if (id < 0 || id >= c.pages) {
+        if (lane == 0) set_status(AIB_DEV_BAD_PAGE);
+      } else {
+        row = id * c.page_stride + (p & ((1 << c.page_shift) - 1)) * c.row_stride;
+      }
     }
   }
-  const int nv = H + 2 * c.KV, v0 = static_cast<int>(w % parts) * per, v1 = min(nv, v0 + per);
-  for (int h0 = v0; h0 < v1; h0 += kAppBatch) {
-    float x[kAppBatch][2 * PER];
+  float cs[4] = {1.0f, 1.0f, 1.0f, 1.0f}, sn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (inv && v0 < H + KV) {  // the warp's groups share the four angles
+    constexpr int PER = 4 / VPW;
+    float ca[PER], sa[PER];
 #pragma unroll
-    for (int i = 0; i < kAppBatch; ++i) {
-      const int h = h0 + i;
-      if (h >= v1) break;
-      const E* src;
-      int vec;
-      if (h < H) {
-        src = q.p + t * q.ts + h * q.hs;
-        vec = q.vec;
-      } else if (h < H + c.KV) {
-        src = k.p + t * k.ts + (h - H) * k.hs;
-        vec = k.vec;
-      } else {
-        src = v.p + t * v.ts + (h - H - c.KV) * v.hs;
-        vec = v.vec;
-      }
-      load_per<PER>(src + r, vec, x[i]);
-      load_per<PER>(src + r + HALF, vec, x[i] + PER);
+    for (int i = 0; i < PER; ++i) {
+      float mine = f[i];
+#pragma unroll
+      for (int s = 1; s < VPW; ++s) mine = sub == s ? f[s * PER + i] : mine;
+      rotation(p, mine, &ca[i], &sa[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kAppBatch; ++i) {
-      const int h = h0 + i;
-      if (h >= v1) break;
-      float* a = x[i];
-      float* z = x[i] + PER;
-      const bool isq = h < H, isv = h >= H + c.KV;
-      if (!isv) {
-        const uint16_t* wn = isq ? qn : kn;
+    for (int i = 0; i < 4; ++i) {
+      cs[i] = __shfl_sync(0xffffffffu, ca[i % PER], i / PER * LPV + lane % LPV);
+      sn[i] = __shfl_sync(0xffffffffu, sa[i % PER], i / PER * LPV + lane % LPV);
+    }
+  }
+  float ac[4], as[4], zc[4], zs[4];  // weight times cosine or sine, of the first half's and of the second's elements
+  int kind = -1;
+  for (int h0 = v0; h0 < v1;) {
+    const int stop = stop_of(h0), now = h0 < H ? 0 : (h0 < H + KV ? 1 : 2);
+    float y[kAppSteps][8];
+    load(stop, y);
+    const uint16_t* wn = now == 0 ? qn : kn;
+    if (now != kind && now != 2) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float wa = wn ? bf16_to_f32(wn[r + j]) : 1.0f, wz = wn ? bf16_to_f32(wn[r + j + HALF]) : 1.0f;
+        ac[j] = wa * cs[j];
+        as[j] = wa * sn[j];
+        zc[j] = wz * cs[j];
+        zs[j] = wz * sn[j];
+      }
+    }
+    kind = now;
+#pragma unroll
+    for (int i = 0; i < kAppSteps; ++i) {
+      const int h = h0 + sub + i * VPW;
+      const bool mine = h < stop;
+      float4 lo = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]), hi = make_float4(x[i][4], x[i][5], x[i][6], x[i][7]);
+      if (now != 2) {
+        float rs = 1.0f;
         if (wn) {
           float ss = 0.0f;
 #pragma unroll
-          for (int j = 0; j < 2 * PER; ++j) ss += x[i][j] * x[i][j];
-          const float rs = rsqrtf(warp_sum(ss) / static_cast<float>(HD) + eps);
+          for (int j = 0; j < 8; ++j) ss += x[i][j] * x[i][j];
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            a[j] = bf16_to_f32(wn[r + j]) * (a[j] * rs);
-            z[j] = bf16_to_f32(wn[r + j + HALF]) * (z[j] * rs);
-          }
+          for (int o = LPV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          rs = rsqrtf(ss * (1.0f / HD) + eps);
         }
-        if (inv) {
+        float a[4], z[4];
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const float lo = a[j], hi = z[j];
-            a[j] = lo * cs[j] - hi * sn[j];
-            z[j] = hi * cs[j] + lo * sn[j];
-          }
+        for (int j = 0; j < 4; ++j) {
+          a[j] = rs * (x[i][j] * ac[j] - x[i][4 + j] * zs[j]);
+          z[j] = rs * (x[i][4 + j] * zc[j] + x[i][j] * as[j]);
         }
+        lo = make_float4(a[0], a[1], a[2], a[3]);
+        hi = make_float4(z[0], z[1], z[2], z[3]);
       }
-      if (isq) {
-        E* dst = qo.p + t * qo.ts + h * qo.hs;
-        store_per<PER>(dst + r, qo.vec, a);
-        store_per<PER>(dst + r + HALF, qo.vec, z);
+      if (!mine) continue;
+      if (now == 0) {
+        E* dst = qo.p + t * qo.ts + h * qo.hs + r;
+        store4(dst, lo, VEC);
+        store4(dst + HALF, hi, VEC);
       } else if (row >= 0) {
-        uint16_t* dst = isv ? c.v + row + (h - H - c.KV) * c.head_stride : c.k + row + (h - H) * c.head_stride;
-        store_per<PER>(dst + r, 1, a);
-        store_per<PER>(dst + r + HALF, 1, z);
+        uint16_t* dst = now == 1 ? c.k + row + (h - H) * c.head_stride + r : c.v + row + (h - H - KV) * c.head_stride + r;
+        store4(dst, lo, true);
+        store4(dst + HALF, hi, true);
       }
     }
+#pragma unroll
+    for (int i = 0; i < kAppSteps; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = y[i][j];
+    h0 = stop;
   }
 }
 
@@ -329,21 +377,6 @@ AIB_DEV void add4(float4& a, float w, float4 x) {
   a.z += w * x.z;
   a.w += w * x.w;
 }
-AIB_DEV void store4(float* p, float4 a, bool vec) {
-  if (vec) {
-    *reinterpret_cast<float4*>(p) = a;
-  } else {
-    p[0] = a.x, p[1] = a.y, p[2] = a.z, p[3] = a.w;
-  }
-}
-AIB_DEV void store4(uint16_t* p, float4 a, bool vec) {
-  const uint32_t lo = bf16x2_rn(a.x, a.y), hi = bf16x2_rn(a.z, a.w);
-  if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
-  } else {
-    p[0] = lo & 0xFFFF, p[1] = lo >> 16, p[2] = hi & 0xFFFF, p[3] = hi >> 16;
-  }
-}
 AIB_DEV float lse_of(float M, float L) {
   return M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
@@ -371,7 +404,7 @@ struct Shared {
 template <int HD, typename E>
 __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int pages, int KV,
-                int page_shift, const int32_t* __restrict__ table, int table_ld, int room,
+                int page_shift, const int32_t* __restrict__ table, long long table_ld, int room,
                 const int64_t* __restrict__ pos, int B, int H, const E* __restrict__ q, long long q_ld,
                 E* __restrict__ out, long long out_ld, float* __restrict__ lse, long long window, float scale, int* cnt,
                 float* parts_ws) {
@@ -471,7 +504,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
         k.row = a & ((1 << page_shift) - 1);
         if (r0 < r1) {
           k.rows = (0xffffffffu >> (32 - (r1 - r0))) << r0;
-          k.id = table[static_cast<long long>(P.b) * table_ld + (a >> page_shift)];
+          k.id = table[P.b * table_ld + (a >> page_shift)];
         }
       }
       return k;
@@ -556,11 +589,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
       const E* qr = q + C.b * q_ld + static_cast<long long>(h0 + min(g, nh - 1)) * HD + 2 * t;
 #pragma unroll
       for (int s = 0; s < NT; ++s) {
-        float x[4];
-        load_per<1>(qr + 16 * s, 0, x);
-        load_per<1>(qr + 16 * s + 1, 0, x + 1);
-        load_per<1>(qr + 16 * s + 8, 0, x + 2);
-        load_per<1>(qr + 16 * s + 9, 0, x + 3);
+        const float x[4] = {to_f32(qr[16 * s]), to_f32(qr[16 * s + 1]), to_f32(qr[16 * s + 8]), to_f32(qr[16 * s + 9])};
         uint32_t w0[PQ], w1[PQ];
         split_pair<PQ>(x[0], x[1], w0);
         split_pair<PQ>(x[2], x[3], w1);
@@ -672,8 +701,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
 #pragma unroll
             for (int d = 0; d < NT; ++d) {
               const float x = M == -INFINITY ? 0.0f : acc[d][hh] * r, y = M == -INFINITY ? 0.0f : acc[d][2 + hh] * r;
-              store_per<1>(o + h * HD + d * 16, 0, &x);
-              store_per<1>(o + h * HD + d * 16 + 8, 0, &y);
+              from_f32(x, o + h * HD + d * 16);
+              from_f32(y, o + h * HD + d * 16 + 8);
             }
             if (lse && g == 0) lse[static_cast<long long>(C.b) * H + h0 + h] = lse_of(M, L);
           }
@@ -871,8 +900,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     int lo, hi;
     span(pos, b, room, window, &lo, &hi);
     if (hi > lo) continue;
-    const float zero = 0.0f;
-    for (int i = threadIdx.x; i < H * HD; i += Y::kThreads) store_per<1>(out + b * out_ld + i, 0, &zero);
+    for (int i = threadIdx.x; i < H * HD; i += Y::kThreads) from_f32(0.0f, out + b * out_ld + i);
     if (lse)
       for (int h = threadIdx.x; h < H; h += Y::kThreads) lse[static_cast<long long>(b) * H + h] = -INFINITY;
   }
@@ -893,27 +921,31 @@ static int check_kv(const char* what, const aib_paged_kv* c, Kv* o) {
 }
 
 template <typename E>
-static Rows<E> rows_of(const aib_rows* r) {
-  if (!r) return Rows<E>{nullptr, 0, 0, 0};
-  const bool vec = !(reinterpret_cast<uintptr_t>(r->p) % (2 * sizeof(E))) && !((r->token_stride | r->head_stride) & 1);
-  return Rows<E>{static_cast<E*>(r->p), r->token_stride, r->head_stride, vec ? 1 : 0};
+static bool vec_rows(const Rows<E>& r) {  // whether four elements may be read at once
+  return !r.p || (!(reinterpret_cast<uintptr_t>(r.p) % (4 * sizeof(E))) && !((r.ts | r.hs) & 3));
 }
 
 template <typename E>
-static int append(const Kv& c, int HD, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
-                  const int32_t* cu, int B, int T, int H, const aib_rows* q, const aib_rows* k, const aib_rows* v,
-                  const aib_rows* qo, const uint16_t* qn, const uint16_t* kn, const float* inv, float eps,
-                  cudaStream_t s) {
+static int append(const Kv& c, int HD, const int32_t* table, long long table_ld, int max_pages, const int64_t* pos,
+                  const int32_t* cu, int B, int T, int H, Rows<const E> q, Rows<const E> k, Rows<const E> v, Rows<E> qo,
+                  const uint16_t* qn, const uint16_t* kn, const float* inv, float eps, cudaStream_t s) {
   const int nv = H + 2 * c.KV;
-  const int parts = 1, per = nv;
+  // A token's vectors go to as few warps as fill the GPU four times over (eight CTAs of eight warps an SM): a warp pays
+  // for its token's angles once, but one warp alone is as slow as its loads one after the other.
+  const int batch = kAppSteps * 256 / HD;
+  const long long want = 4LL * 64 * sm_count();
+  int parts = static_cast<int>(std::min<long long>((want + T - 1) / T, (nv + batch - 1) / batch));
+  const int per = ((nv + parts - 1) / parts + batch - 1) / batch * batch;
+  parts = (nv + per - 1) / per;
   const long long warps = static_cast<long long>(T) * parts;
   const dim3 grid(static_cast<unsigned>((warps + kAppWarps - 1) / kAppWarps));
   auto go = [&](auto kernel) {
     return launch(kernel, grid, dim3(32 * kAppWarps), 0, s, "aib_paged_append", c, table, table_ld, max_pages, pos, cu,
-                  B, T, H, rows_of<const E>(q), rows_of<const E>(k), rows_of<const E>(v), rows_of<E>(qo), qn, kn, inv,
-                  eps, parts, per);
+                  B, T, H, q, k, v, qo, qn, kn, inv, eps, parts, per);
   };
-  return HD == 128 ? go(append_kernel<128, E>) : go(append_kernel<64, E>);
+  if (vec_rows(q) && vec_rows(k) && vec_rows(v) && vec_rows(qo))
+    return HD == 128 ? go(append_kernel<128, E, true>) : go(append_kernel<64, E, true>);
+  return HD == 128 ? go(append_kernel<128, E, false>) : go(append_kernel<64, E, false>);
 }
 
 static int max_grid() { return std::min(kMaxGrid, sm_count()); }
@@ -946,11 +978,18 @@ static int pool_map(CUtensorMap* map, const uint16_t* p, const aib_paged_kv* c) 
 }
 
 template <int HD, typename E>
-static int attend(const aib_paged_kv* c, const int32_t* table, int table_ld, int room, const int64_t* pos, int B, int H,
+static int attend(const aib_paged_kv* c, const int32_t* table, long long table_ld, int room, const int64_t* pos, int B, int H,
                   const void* q, long long q_ld, void* out, long long out_ld, float* lse, long long window, float scale,
                   void* ws, cudaStream_t s) {
   const int G = H / c->KV, tiles = (G + GT - 1) / GT;
-  int rc = allow_smem(attn_kernel<HD, E>, smem_bytes<HD>());
+  // the shared-memory limit is raised once on each device (the query behind it costs more than the rest of a call)
+  static std::atomic<uint64_t> raised{0};
+  int dev = 0, rc = AIB_OK;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !(raised.load(std::memory_order_relaxed) >> dev & 1)) {
+    rc = allow_smem(attn_kernel<HD, E>, smem_bytes<HD>());
+    if (!rc && dev < 64) raised.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   CUtensorMap kmap, vmap;
   if (!rc) rc = pool_map(&kmap, c->k, c);
   if (!rc) rc = pool_map(&vmap, c->v, c);
@@ -972,26 +1011,35 @@ using namespace aib;
 
 extern "C" {
 
-int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
-                     const int32_t* cu, int B, int T, int H, const aib_rows* q, const aib_rows* k, const aib_rows* v,
-                     const aib_rows* q_out, int dtype, const uint16_t* qn, const uint16_t* kn, const float* inv,
-                     float eps, void* stream) {
+int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t table_ld, int max_pages,
+                     const int64_t* pos, const int32_t* cu, int B, int T, int H, const void* q, int64_t q_ts,
+                     int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                     void* q_out, int64_t qo_ts, int64_t qo_hs, int dtype, const uint16_t* qn, const uint16_t* kn,
+                     const float* inv, float eps, void* stream) {
   paged::Kv c;
   const int rc = paged::check_kv("aib_paged_append", cache, &c);
   if (rc) return rc;
-  if (!table || !pos || !k || !v || !k->p || !v->p || B <= 0 || T <= 0 || max_pages <= 0 || table_ld < 0 ||
-      (dtype != 0 && dtype != 1))
+  if (!table || !pos || !k || !v || B <= 0 || T <= 0 || max_pages <= 0 || table_ld < 0 || (dtype != 0 && dtype != 1))
     return fail(AIB_EINVAL, "aib_paged_append: bad arguments");
   if (!cu && T != B) return fail(AIB_EINVAL, "aib_paged_append: without cu, T must be B (T=%d B=%d)", T, B);
-  if (H < 0 || (H > 0) != (q && q->p) || (H > 0) != (q_out && q_out->p))
+  if (H < 0 || (H > 0) != (q != nullptr) || (H > 0) != (q_out != nullptr))
     return fail(AIB_EINVAL, "aib_paged_append: q and q_out go with H > 0");
-  if (static_cast<long long>(T) * (H + 2 * c.KV) > 0x7fffffffLL)
+  const size_t es = dtype == 0 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(q_out)) % es)
+    return fail(AIB_EINVAL, "aib_paged_append: rows must be aligned to their elements");
+  if (static_cast<long long>(T) * (H + 2LL * c.KV) > 0x7fffffffLL)
     return fail(AIB_ENOTSUP, "aib_paged_append: T * (H + 2 KV) must fit 31 bits");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == 0 ? paged::append<float>(c, cache->HD, table, table_ld, max_pages, pos, cu, B, T, H, q, k, v, q_out,
-                                           qn, kn, inv, eps, s)
-                    : paged::append<uint16_t>(c, cache->HD, table, table_ld, max_pages, pos, cu, B, T, H, q, k, v,
-                                              q_out, qn, kn, inv, eps, s);
+  auto go = [&](auto e) {
+    using E = decltype(e);
+    return paged::append<E>(c, cache->HD, table, table_ld, max_pages, pos, cu, B, T, H,
+                            paged::Rows<const E>{static_cast<const E*>(q), q_ts, q_hs},
+                            paged::Rows<const E>{static_cast<const E*>(k), k_ts, k_hs},
+                            paged::Rows<const E>{static_cast<const E*>(v), v_ts, v_hs},
+                            paged::Rows<E>{static_cast<E*>(q_out), qo_ts, qo_hs}, qn, kn, inv, eps, s);
+  };
+  return dtype == 0 ? go(float()) : go(uint16_t());
 }
 
 size_t aib_paged_attn_workspace(int B, int H, int KV, int HD) {
@@ -999,8 +1047,8 @@ size_t aib_paged_attn_workspace(int B, int H, int KV, int HD) {
   return paged::attn_ws_bytes(HD);
 }
 
-int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
-                   int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,
+int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t table_ld, int max_pages,
+                   const int64_t* pos, int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,
                    int64_t window, float scale, void* ws, size_t ws_bytes, void* stream) {
   paged::Kv c;
   const int rc = paged::check_kv("aib_paged_attn", cache, &c);

@@ -17,7 +17,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import PagedKv, Rows, ptr, stream_ptr
+from ._lib import PagedKv
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -43,30 +43,41 @@ class Cache:
         self.ref = C.byref(self.desc)
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def _check_table(what, cache, table, pos):
-    B = pos.shape[0]
-    if table.dim() != 2 or table.shape[0] != B or table.dtype != torch.int32 or table.device != cache.device or \
-            table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{what}: table must be int32 [B, width] on the cache's device")
-    if pos.dim() != 1 or pos.dtype != torch.int64 or pos.device != cache.device or (B > 1 and pos.stride(0) != 1):
+    """Returns the batch size and the table's width and row stride."""
+    if pos.dim() != 1 or pos.dtype != torch.int64 or pos.device != cache.device or not pos.is_contiguous():
         raise ValueError(f"{what}: pos must be int64 [B] on the cache's device")
-    return B
+    B = pos.shape[0]
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or shape[0] != B or shape[1] < 1 or (shape[1] > 1 and stride[1] != 1) or \
+            table.dtype != torch.int32 or table.device != cache.device:
+        raise ValueError(f"{what}: table must be int32 [B, width] on the cache's device")
+    return B, shape[1], stride[0]
 
 
-def _rows(what, t, T, heads, HD, dtype, device):
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != HD or (heads and t.shape[1] != heads) or t.dtype != dtype or \
-            t.device != device or t.stride(2) != 1:
-        raise ValueError(f"append: {what} must be [T, heads, HD] rows like k on the cache's device")
-    return Rows(t.data_ptr(), t.stride(0), t.stride(1))
+def _rows(what, t, shape, dtype, device):
+    """Returns the address and the token and head strides of rows [T, heads, HD]."""
+    stride = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.device != device or stride[2] != 1:
+        raise ValueError(f"append: {what} must be {dtype} {list(shape)} rows on the cache's device")
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _norm(what, w, HD, device):
-    if w is None:
+def _vector(what, t, n, dtypes, device):
+    if t is None:
         return None
-    if w.dtype not in (torch.bfloat16, torch.int16, torch.uint16) or w.shape != (HD,) or w.device != device or \
-            w.stride(0) != 1:
-        raise ValueError(f"append: {what} must be bf16 [HD] on the cache's device")
-    return ptr(w)
+    if t.dtype not in dtypes or t.shape != (n,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"append: {what} must be {dtypes[0]} [{n}] on the cache's device")
+    return t.data_ptr()
+
+
+_NORM = (torch.bfloat16, torch.int16, torch.uint16)
+_F32 = (torch.float32,)
+_I32 = (torch.int32,)
 
 
 def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=None, inv=None, eps=1e-6):
@@ -75,32 +86,28 @@ def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=Non
     cu[B] on are left alone. Without cu there is one token per sequence (T == B). qn / kn: q / k norm weights (bf16
     [HD]); inv: fp32 [HD/2] rotation frequencies (None: no rotation, for keys that are rotated already). q [T, H, HD]
     is normed and rotated into q_out (q_out may be q itself). No two tokens may share a cache row."""
-    B = _check_table("append", cache, table, pos)
-    if k.dtype not in _DT:
-        raise ValueError("append: rows must be fp32 or bf16")
-    T, HD, dev, dt = k.shape[0], cache.HD, cache.device, k.dtype
-    if T == 0 or B == 0:
-        return q_out
-    kr, vr = _rows("k", k, T, cache.KV, HD, dt, dev), _rows("v", v, T, cache.KV, HD, dt, dev)
+    B, width, ld = _check_table("append", cache, table, pos)
+    dt = k.dtype
+    if dt not in _DT or k.dim() != 3:
+        raise ValueError("append: rows must be fp32 or bf16 [T, heads, HD]")
+    T, KV, HD, dev = k.shape[0], cache.KV, cache.HD, cache.device
     if (q is None) != (q_out is None):
         raise ValueError("append: q and q_out go together")
-    H, qr, qo = 0, None, None
-    if q is not None:
-        qr, qo = _rows("q", q, T, 0, HD, dt, dev), _rows("q_out", q_out, T, q.shape[1], HD, dt, dev)
+    kr, vr = _rows("k", k, (T, KV, HD), dt, dev), _rows("v", v, (T, KV, HD), dt, dev)
+    H, qr, qo = 0, (None, 0, 0), (None, 0, 0)
+    if q is not None and q.dim() == 3 and q.shape[1]:
         H = q.shape[1]
-        qr, qo = (C.byref(qr), C.byref(qo)) if H else (None, None)
-    if cu is None:
-        if T != B:
-            raise ValueError("append: without cu there must be one token per sequence")
-    elif cu.dtype != torch.int32 or cu.shape != (B + 1,) or cu.device != dev or cu.stride(0) != 1:
-        raise ValueError("append: cu must be int32 [B + 1] on the cache's device")
-    if inv is not None and (inv.dtype != torch.float32 or inv.shape != (HD // 2,) or inv.device != dev or
-                            inv.stride(0) != 1):
-        raise ValueError("append: inv must be fp32 [HD/2] on the cache's device")
-    with _lib.device_of(k):
-        _lib.call("aib_paged_append", cache.ref, ptr(table), table.stride(0), table.shape[1], ptr(pos), ptr(cu), B, T, H,
-                  qr, C.byref(kr), C.byref(vr), qo, _DT[dt], _norm("qn", qn, HD, dev), _norm("kn", kn, HD, dev),
-                  ptr(inv), eps, stream_ptr())
+        qr, qo = _rows("q", q, (T, H, HD), dt, dev), _rows("q_out", q_out, (T, H, HD), dt, dev)
+    cu_at = _vector("cu", cu, B + 1, _I32, dev)
+    if cu is None and T != B:
+        raise ValueError("append: without cu there must be one token per sequence")
+    qn_at, kn_at = _vector("qn", qn, HD, _NORM, dev), _vector("kn", kn, HD, _NORM, dev)
+    inv_at = _vector("inv", inv, HD // 2, _F32, dev)
+    if T == 0 or B == 0:
+        return q_out
+    with _lib.on_device(dev.index) as stream:
+        _lib.call("aib_paged_append", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), cu_at, B, T, H, *qr, *kr,
+                  *vr, *qo, _DT[dt], qn_at, kn_at, inv_at, eps, stream)
     return q_out
 
 
@@ -117,33 +124,36 @@ def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws
     of them. out: [B, H, HD] like q (allocated when None); lse: optional fp32 [B, H], the log of the summed
     exponentials; scale: default HD ** -0.5; ws: from `workspace` (a fresh one per call when None). A row that attends
     nothing gives zeros and lse -inf. Returns out."""
-    B = _check_table("attention", cache, table, pos)
-    HD, dev = cache.HD, cache.device
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != HD or q.dtype not in _DT or q.device != dev:
+    B, width, ld = _check_table("attention", cache, table, pos)
+    HD, dev, dt = cache.HD, cache.device, q.dtype
+    shape = q.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != HD or dt not in _DT or q.device != dev:
         raise ValueError("attention: q must be fp32 or bf16 [B, H, HD] on the cache's device")
-    H = q.shape[1]
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    if B == 0 or H == 0:
-        return out
+    H = shape[1]
     if H % cache.KV:
         raise ValueError("attention: the query heads must be a multiple of the key heads")
-    if out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+    elif out.shape != shape or out.dtype != dt or out.device != dev:
         raise ValueError("attention: out must have the shape, type and device of q")
-    for t in (q, out):
-        if t.stride(2) != 1 or (H > 1 and t.stride(1) != HD):
-            raise ValueError("attention: the heads of a row must be contiguous")
-    if B > 1 and out.stride(0) < H * HD:
+    q_st, out_st = q.stride(), out.stride()
+    if q_st[2] != 1 or out_st[2] != 1 or (H > 1 and (q_st[1] != HD or out_st[1] != HD)):
+        raise ValueError("attention: the heads of a row must be contiguous")
+    if B > 1 and out_st[0] < H * HD:
         raise ValueError("attention: the rows of out must be apart")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or lse.device != dev or
                             not lse.is_contiguous()):
         raise ValueError("attention: lse must be fp32 [B, H] on the cache's device")
     if window < 0:
         raise ValueError("attention: window must not be negative")
-    with _lib.device_of(q):
-        if ws is None:
-            ws = workspace(B, H, cache)
-        _lib.call("aib_paged_attn", cache.ref, ptr(table), table.stride(0), table.shape[1], ptr(pos), B, H, ptr(q),
-                  q.stride(0), ptr(out), out.stride(0), _DT[q.dtype], ptr(lse), window,
-                  HD ** -0.5 if scale is None else scale, ptr(ws), ws.numel(), stream_ptr())
+    if B == 0 or H == 0:
+        return out
+    if ws is None:
+        ws = workspace(B, H, cache)
+    elif ws.dtype != torch.uint8 or ws.device != dev or not ws.is_contiguous():
+        raise ValueError("attention: ws must come from paged.workspace on the cache's device")
+    with _lib.on_device(dev.index) as stream:
+        _lib.call("aib_paged_attn", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), B, H, q.data_ptr(), q_st[0],
+                  out.data_ptr(), out_st[0], _DT[dt], _addr(lse), window, HD ** -0.5 if scale is None else scale,
+                  ws.data_ptr(), ws.numel(), stream)
     return out

@@ -46,52 +46,63 @@ def adjust(logits, out=None, prior=None, repetition=None, presence=None, frequen
            mask=None):
     """Penalties, biases and grammar masks of a batch of requests, each row with its own parameters (see
     aib_adjust_logits in include/ai_b200.h for the formula): logits [B, V] fp32 or bf16 CUDA rows -> out (default: in
-    place). repetition (> 0) / presence / frequency: fp32 [B] over the ids of prior (int32 [B, P], P <= 65535, -1 =
+    place). repetition (> 0) / presence / frequency: fp32 [B] over the ids of prior (int32 [B, P], P <= 32767, -1 =
     empty); bias_ids int32 / bias fp32 [B, n], n <= 1024 (biases of an id listed twice add up, ids outside the
     vocabulary are ignored); mask int32 [B, ceil(V/32)], 1 = allowed. prior, biases and mask may be expanded from one
     row. Returns out."""
-    if out is None:
-        out = logits
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or not logits.is_cuda:
         raise ValueError("adjust: logits must be fp32 or bf16 CUDA rows [B, V]")
-    B, V = logits.shape
-    if B == 0 or V == 0:
-        return out
-    dev = logits.device
-    ld, out_ld = logits.stride(0), out.stride(0)
-    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
-        raise ValueError("adjust: out must have the shape, type and device of logits")
-    if logits.stride(1) != 1 or out.stride(1) != 1 or (B > 1 and out_ld < V):
-        raise ValueError("adjust: rows must be contiguous and the rows of out apart")
-    if out is not logits:
-        es = logits.element_size()
-        a, b = logits.data_ptr(), out.data_ptr()
-        if a < b + ((B - 1) * out_ld + V) * es and b < a + ((B - 1) * ld + V) * es and (a, ld) != (b, out_ld):
+    shape, dt, dev = logits.shape, logits.dtype, logits.device
+    B, V = shape
+    ld, step = logits.stride()
+    at = out_at = logits.data_ptr()
+    if out is None or out is logits:
+        out, out_ld = logits, ld
+    else:
+        if out.shape != shape or out.dtype != dt or out.device != dev:
+            raise ValueError("adjust: out must have the shape, type and device of logits")
+        out_ld, out_step = out.stride()
+        step = max(step, out_step)
+        out_at, es = out.data_ptr(), logits.element_size()
+        if at < out_at + ((B - 1) * out_ld + V) * es and out_at < at + ((B - 1) * ld + V) * es and \
+                (at, ld) != (out_at, out_ld):
             raise ValueError("adjust: out must be logits itself or share no memory with it")
-    args = []
-    for name, t, dtype in (("prior", prior, torch.int32), ("bias_ids", bias_ids, torch.int32),
-                           ("bias", bias, torch.float32), ("mask", mask, torch.int32)):
-        if t is None:
-            args.append((None, 0, 0))
-            continue
-        if t.dim() != 2 or t.shape[0] != B or t.dtype != dtype or t.device != dev or (t.shape[1] > 1 and
-                                                                                     t.stride(1) != 1):
-            raise ValueError(f"adjust: {name} must be {dtype} [B, n] rows on the logits' device")
-        args.append((ptr(t) if t.shape[1] else None, t.stride(0), t.shape[1]))
-    (pr, pr_ld, n_prior), (bi, bi_ld, nb), (bv, bv_ld, nv), (mk, mk_ld, nm) = args
+    if (V > 1 and step != 1) or (B > 1 and out_ld < V):
+        raise ValueError("adjust: rows must be contiguous and the rows of out apart")
+    prior_at, prior_ld, n_prior = _side("prior", prior, B, torch.int32, dev)
+    ids_at, ids_ld, nb = _side("bias_ids", bias_ids, B, torch.int32, dev)
+    bias_at, bias_ld, nv = _side("bias", bias, B, torch.float32, dev)
+    mask_at, mask_ld, words = _side("mask", mask, B, torch.int32, dev)
     if nb != nv:
         raise ValueError("adjust: bias_ids and bias go together")
-    if mask is not None and nm != (V + 31) // 32:
+    if mask is not None and words != (V + 31) // 32:
         raise ValueError("adjust: mask must have ceil(V/32) words a row")
-    for name, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (B,) or t.device != dev or
-                              (B > 1 and t.stride(0) != 1)):
-            raise ValueError(f"adjust: {name} must be fp32 [B] on the logits' device")
-    with _lib.device_of(logits):
-        _lib.call("aib_adjust_logits", ptr(logits), ld, ptr(out), out_ld, int(logits.dtype == torch.bfloat16), B, V, pr,
-                  pr_ld, n_prior, ptr(repetition), ptr(presence), ptr(frequency), bi, bi_ld, bv, bv_ld, nb, mk, mk_ld,
-                  stream_ptr())
+    rep_at, pres_at, freq_at = (_per_row(n, t, B, dev) for n, t in (("repetition", repetition), ("presence", presence),
+                                                                    ("frequency", frequency)))
+    if B == 0 or V == 0:
+        return out
+    with _lib.on_device(dev.index) as stream:
+        _lib.call("aib_adjust_logits", at, ld, out_at, out_ld, int(dt == torch.bfloat16), B, V, prior_at, prior_ld,
+                  n_prior, rep_at, pres_at, freq_at, ids_at, ids_ld, bias_at, bias_ld, nb, mask_at, mask_ld, stream)
     return out
+
+
+def _side(what, t, B, dtype, device):
+    """Address, row stride and width of an optional [B, n] argument of `adjust`."""
+    if t is None:
+        return None, 0, 0
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or shape[0] != B or t.dtype != dtype or t.device != device or (shape[1] > 1 and stride[1] != 1):
+        raise ValueError(f"adjust: {what} must be {dtype} [B, n] rows on the logits' device")
+    return (t.data_ptr() if shape[1] else None), stride[0], shape[1]
+
+
+def _per_row(what, t, B, device):
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.shape != (B,) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"adjust: {what} must be fp32 [B] on the logits' device")
+    return t.data_ptr()
 
 
 def sample(logits, temperature=0.0, top_p=1.0, top_k=0, us=None, prior=None, mask=None, repetition_penalty=1.0,

@@ -240,21 +240,18 @@ typedef struct aib_paged_kv {
   int64_t page_stride, head_stride, row_stride;
   int32_t pages, page, KV, HD;
 } aib_paged_kv;
-/* Rows [T, heads, HD], elements contiguous along HD; strides in elements. */
-typedef struct aib_rows {
-  void* p;
-  int64_t token_stride, head_stride;
-} aib_rows;
 /* Appends T new tokens: k, v rows go to their pages as bf16, q rows to q_out (q, q_out: H heads, or H == 0 and NULL).
  * Sequence b's tokens are rows cu[b] .. cu[b + 1] - 1 (int32 [B + 1], ascending), its first at position pos[b]; rows
  * from cu[B] on, and the rows of a sequence with pos[b] < 0, are left alone. cu NULL: one token per sequence (T == B).
  * q and k: RMSNorm over HD with weights qn / kn (bf16 [HD]; NULL: none), then the half-split rotation by
  * position * inv[r] (fp32 [HD/2]; NULL: none), as aib_qk_rope_cache, with the angle formed in 64 bits.
- * dtype of q, k, v, q_out: 0 fp32, 1 bf16. q_out may be q itself. No two tokens of a call may share a cache row. */
-int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
-                     const int32_t* cu, int B, int T, int H, const aib_rows* q, const aib_rows* k, const aib_rows* v,
-                     const aib_rows* q_out, int dtype, const uint16_t* qn, const uint16_t* kn, const float* inv,
-                     float eps, void* stream);
+ * q, k, v, q_out: rows [T, heads, HD], elements contiguous along HD, token stride *_ts and head stride *_hs in
+ * elements; dtype 0 fp32, 1 bf16. q_out may be q itself, else it shares no memory with the inputs. No two tokens of a call may share a cache row. */
+int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t table_ld, int max_pages,
+                     const int64_t* pos, const int32_t* cu, int B, int T, int H, const void* q, int64_t q_ts,
+                     int64_t q_hs, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs,
+                     void* q_out, int64_t qo_ts, int64_t qo_hs, int dtype, const uint16_t* qn, const uint16_t* kn,
+                     const float* inv, float eps, void* stream);
 /* Attention of one new token per sequence, its own k and v already in the cache: q [B, H, HD] (normed and rotated;
  * rows at q_ld) attends positions max(0, pos[b] - window + 1) .. pos[b] (window 0: 0 .. pos[b]); out [B, H, HD] (rows
  * at out_ld), lse fp32 [B, H] or NULL = log of the sum of exp(scale * q.k). A row that attends nothing gives zeros and
@@ -262,8 +259,8 @@ int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int table_
  * ws: aib_paged_attn_workspace(...) bytes, 16-byte aligned, zero-filled once (left zeroed where it must be); calls that
  * may overlap on the GPU need separate ones. B <= 4096. */
 size_t aib_paged_attn_workspace(int B, int H, int KV, int HD);
-int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int table_ld, int max_pages, const int64_t* pos,
-                   int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,
+int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t table_ld, int max_pages,
+                   const int64_t* pos, int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,
                    int64_t window, float scale, void* ws, size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------- tensor parallelism ---- */
@@ -310,7 +307,7 @@ int aib_sample(const float* logits, int B, int V, int ld, const aib_sample_param
  * fp32 / 1 bf16, in fp32 and rounded once: penalties as aib_sample's over the row's prior ids (repetition over their
  * set, then - (frequency * count + presence)); + the sum, in list order, of the row's biases of that id; -inf where the
  * mask bit (bit j of word w = token 32w + j) is 0. repetition (> 0), presence, frequency: fp32 [B] or NULL (1, 0, 0);
- * prior int32 [B, n_prior] (at most 65535), bias_ids int32 / bias fp32 [B, n_bias] (at most 1024): ids outside [0, V)
+ * prior int32 [B, n_prior] (at most 32767), bias_ids int32 / bias fp32 [B, n_bias] (at most 1024): ids outside [0, V)
  * are ignored; mask int32 [B, ceil(V/32)] or NULL. The row strides *_ld of prior, biases and mask may be 0 (one row
  * for all). out may be logits itself (same ld), else they share no memory. */
 int aib_adjust_logits(const void* logits, int64_t ld, void* out, int64_t out_ld, int dtype, int B, int V,

@@ -394,7 +394,7 @@ ADJUST = [  # B, V, prior ids, biases, mask, logits row stride beyond V, out row
     (5, 4099, 1, 1, False, 0, 5),
     (2, 50257, 600, 64, True, 0, 0),
     (2, 151936, 5000, 1024, True, 64, 0),
-    (1, 9000, 65535, 7, False, 0, 0),
+    (1, 9000, 32767, 7, False, 0, 0),
     (17, 8192, 0, 33, False, 0, 0),
     (4, 40000, 100, 0, False, 3, 3),
     (300, 77, 9, 4, True, 0, 0),

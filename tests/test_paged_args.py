@@ -27,15 +27,11 @@ A = C.c_void_p(1 << 20)  # stands for a device pointer: never read by a refused 
 
 
 def append(L, c=None, **kw):
-    from ai_b200._lib import Rows
-    a = dict(table=A, ld=4, width=4, pos=A, cu=None, B=2, T=2, H=4, q=Rows(1 << 20, 512, 128),
-             k=Rows(1 << 20, 256, 128), v=Rows(1 << 20, 256, 128), q_out=Rows(1 << 20, 512, 128), dtype=0, qn=None,
-             kn=None, inv=None, eps=1e-6)
+    a = dict(table=A, ld=4, width=4, pos=A, cu=None, B=2, T=2, H=4, q=A, k=A, v=A, q_out=A, dtype=0)
     a.update(kw)
-    ref = lambda r: None if r is None else C.byref(r)  # noqa: E731
     return L.aib_paged_append(C.byref(c or kv()), a["table"], a["ld"], a["width"], a["pos"], a["cu"], a["B"], a["T"],
-                              a["H"], ref(a["q"]), ref(a["k"]), ref(a["v"]), ref(a["q_out"]), a["dtype"], a["qn"],
-                              a["kn"], a["inv"], a["eps"], None)
+                              a["H"], a["q"], 512, 128, a["k"], 256, 128, a["v"], 256, 128, a["q_out"], 512, 128,
+                              a["dtype"], None, None, None, 1e-6, None)
 
 
 def attn(L, c=None, **kw):
@@ -60,7 +56,7 @@ def test_bad_caches_are_refused(L, bad, code):
 
 @pytest.mark.parametrize("bad", [dict(table=None), dict(pos=None), dict(k=None), dict(v=None), dict(B=0), dict(T=0),
                                  dict(T=3), dict(width=0), dict(dtype=2), dict(H=-1), dict(H=0), dict(q=None),
-                                 dict(q_out=None)])
+                                 dict(q_out=None), dict(k=C.c_void_p((1 << 20) + 2))])
 def test_append_refusals(L, bad):
     assert append(L, **bad) == -1 and L.aib_last_error().startswith(b"aib_paged_append")
 
@@ -76,7 +72,7 @@ def test_attention_refusals(L, bad, code):
 @pytest.mark.parametrize("bad,code", [
     (dict(x=None), -1), (dict(out=None), -1), (dict(B=0), -1), (dict(V=0), -1), (dict(dtype=2), -1),
     (dict(out_ld=9), -1), (dict(n_prior=1), -1), (dict(n_bias=1), -1), (dict(n_prior=-1), -1), (dict(ld=-1), -1),
-    (dict(prior=A, n_prior=65536), -4), (dict(ids=A, bias=A, n_bias=1025), -4), (dict(x=C.c_void_p((1 << 20) + 2)), -1)])
+    (dict(prior=A, n_prior=32768), -4), (dict(ids=A, bias=A, n_bias=1025), -4), (dict(x=C.c_void_p((1 << 20) + 2)), -1)])
 def test_adjust_refusals(L, bad, code):
     a = dict(x=A, ld=10, out=A, out_ld=10, dtype=0, B=2, V=10, prior=None, n_prior=0, ids=None, bias=None, n_bias=0)
     a.update(bad)
