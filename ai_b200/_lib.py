@@ -63,6 +63,7 @@ SIGNATURES = {
     "aib_embed": (I32, [P, P, I32, I32, I32, P, P]),
     "aib_step_advance": (I32, [P, P, P, I32, P, I32, P]),
     "aib_batch_advance": (I32, [P, P, P, I32, P]),
+    "aib_batch_advance_prior": (I32, [P, P, P, I32, P, I64, I32, P]),
     "aib_allreduce_oneshot": (I32, [P, I32, I32, P, P, I32, I32, P, P]),
     "aib_attn_workspace": (SZ, [I32, I32, I32, I32, I32]),
     "aib_rope_attn_decode": (I32, [P, P, P, P, P, P, P, P, I32, I32, I32, I32, F32, F32, P, SZ, P]),
@@ -112,8 +113,9 @@ def check(rc, what=""):
 
 
 def call(name, *args):
-    rc = getattr(lib(), name)(*args)
-    check(rc, name)
+    rc = getattr(_lib or lib(), name)(*args)
+    if rc != AIB_OK:
+        check(rc, name)
     return rc
 
 
@@ -144,7 +146,7 @@ class on_device:
         self.new = index
 
     def __enter__(self):
-        self.old = torch.cuda.current_device()
+        self.old = torch._C._cuda_getDevice()
         if self.old != self.new:
             torch.cuda.set_device(self.new)
         return torch._C._cuda_getCurrentRawStream(self.new)

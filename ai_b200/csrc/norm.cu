@@ -76,12 +76,16 @@ __global__ void advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* o
   pdl_trigger();
 }
 
-// Batched decode: sequence b's sampled id becomes its next input and its position advances by one.
-__global__ void batch_advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B) {
+// Batched decode: sequence b's sampled id becomes its next input and its position advances by one; its ring of prior ids
+// (if any) takes the id in.
+__global__ void batch_advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, int32_t* prior,
+                                     long long prior_ld, int n_prior) {
   pdl_wait();
   for (int b = threadIdx.x; b < B; b += blockDim.x) {
-    next_ids[b] = out_ids[b];
-    pos[b] += 1;
+    const int64_t tok = out_ids[b], p = pos[b] + 1;
+    next_ids[b] = tok;
+    if (prior && n_prior > 0 && p >= 0) prior[b * prior_ld + p % n_prior] = static_cast<int32_t>(tok);
+    pos[b] = p;
   }
   pdl_trigger();
 }
@@ -113,9 +117,14 @@ int aib_step_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, in
 }
 
 int aib_batch_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, void* stream) {
-  if (!pos || !next_ids || !out_ids || B <= 0) return fail(AIB_EINVAL, "aib_batch_advance: bad arguments");
-  return launch(norm::batch_advance_kernel, dim3(1), dim3(32), 0, static_cast<cudaStream_t>(stream),
-                "aib_batch_advance", pos, next_ids, out_ids, B);
+  return aib_batch_advance_prior(pos, next_ids, out_ids, B, nullptr, 0, 0, stream);
 }
 
+int aib_batch_advance_prior(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, int32_t* prior,
+                            int64_t prior_ld, int n_prior, void* stream) {
+  if (!pos || !next_ids || !out_ids || B <= 0 || n_prior < 0 || prior_ld < 0)
+    return fail(AIB_EINVAL, "aib_batch_advance: bad arguments");
+  return launch(norm::batch_advance_kernel, dim3(1), dim3(32), 0, static_cast<cudaStream_t>(stream),
+                "aib_batch_advance", pos, next_ids, out_ids, B, prior, static_cast<long long>(prior_ld), n_prior);
+}
 }  // extern "C"

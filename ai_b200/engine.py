@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from .head import Head as Head8, exact_logits
-from . import _lib, wcomp, tkernels, sampler, codecfile, prefill
+from . import _lib, wcomp, tkernels, sampler, codecfile, prefill, paged
 from ._lib import ptr, stream_ptr
 from .model import CONFIGS, Ckpt, RandomWeights, Qwen3Config, check_tp, shard_layer
 
@@ -309,10 +309,9 @@ class Engine:
         self.logits[r0:T].view(rows, self.tp, self.Vs).copy_(
             self.logits_all[:n].view(self.tp, rows, self.Vs).transpose(0, 1))
 
-    def _prefill(self, tokens, pos0, prm, us, penal):
-        """Whole-prompt prefill (the reference's blocked path, core/engine.py:446-487 with kernels/prefill.py):
-        every layer runs over all n prompt rows at once -- tcgen05 GEMMs that read each weight matrix once per
-        token tile, causal flash attention -- then the head picks after the last row. Returns [token]."""
+    def _prompt(self, tokens, pos0):
+        """Every layer over all n prompt rows at once (tcgen05 GEMMs that read each weight matrix once per token tile,
+        causal flash attention), K/V into the cache; leaves the last row in xb[0] and its position in pos."""
         n = len(tokens)
         ids = torch.tensor(tokens, dtype=torch.int64).to(self.device)
         x = torch.empty(n, self.D, device=self.device)
@@ -322,6 +321,11 @@ class Engine:
             prefill.layer(self, l, x, pos0, bufs)
         self.xb[0].copy_(x[n - 1])
         self.pos.fill_(pos0 + n - 1)  # the head step advances it to pos0 + n
+
+    def _prefill(self, tokens, pos0, prm, us, penal):
+        """Whole-prompt prefill (the reference's blocked path, core/engine.py:446-487 with kernels/prefill.py): the
+        layers over the whole prompt, then the head picks after the last row. Returns [token]."""
+        self._prompt(tokens, pos0)
         if prm.temperature > 0:
             self.u[0] = us[0]
         self._pick(1, prm, 1, penal)
@@ -524,11 +528,18 @@ class Engine:
         return self.weight_bytes + self.head_bytes + kv
 
     # ------------------------------------------------------------------------------ batched decode
-    def generate_batch(self, prompts, max_new=256, temperature=0.0, top_p=1.0, top_k=0, seed=None):
+    def generate_batch(self, prompts, max_new=256, temperature=0.0, top_p=1.0, top_k=0, seed=None, page=None, pages=None,
+                       repetition_penalty=1.0, presence_penalty=0.0, frequency_penalty=0.0, logit_bias=None, mask=None):
         """Decode B <= 16 independent sequences together (no reference counterpart: the reference engine decodes
         one sequence). Each prompt is prefilled into its own KV cache; then every step reads each weight matrix
         once for all B tokens. Returns B token lists of max_new tokens each (no early stop at EOS, so the batch
-        stays aligned). Uniform draws come from np.random.default_rng(seed), B per step in sequence order."""
+        stays aligned). Uniform draws come from np.random.default_rng(seed), B per step in sequence order.
+        page: rows per page (a power of two) of a cache in pages instead of one of `maxt` rows for every sequence; it
+        holds `pages` pages (default: what these prompts and max_new need) and the engine keeps it for later calls.
+        Penalties: one number, or one for every prompt, over the most recent 4096 ids of the prompt and its tokens.
+        logit_bias: one {id: bias} (or None) for every prompt. mask: int32 [B, ceil(V/32)] (or one row for all), bit j
+        of word w = token 32w + j may be drawn; or a function of the tokens so far (a list for every prompt) that gives
+        one before every draw, a grammar's state for instance."""
         B = len(prompts)
         if not 1 <= B <= MAXB:
             raise ValueError(f"generate_batch takes 1..{MAXB} prompts")
@@ -538,20 +549,45 @@ class Engine:
             self._validate_process(list(p), 0)
             if len(p) + max_new > self.maxt:
                 raise ValueError(f"prompt + max_new longer than the context {self.maxt}")
-        bt = self._batch(B)
+        adj = Adjustment.of(self, prompts, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, mask)
+        if page is None:
+            if pages is not None:
+                raise ValueError("pages go with a page size")
+            bt = self._batch(B)
+        else:
+            bt = self._paged_batch(B, page, pages, [len(p) + max(1, max_new) for p in prompts])
         prm = sampler.params(temperature, top_k, top_p)
         rng = np.random.default_rng(seed)
         out = [[] for _ in range(B)]
-        for b, p in enumerate(prompts):
-            us = [rng.random()] if temperature > 0 else None
-            out[b].append(bt.prefill(b, list(p), prm, us))
-        for _ in range(max_new - 1):
-            if temperature > 0:
-                bt.u.copy_(torch.from_numpy(rng.random(B)))
-            bt.run(prm)
-            for b, t in enumerate(bt.out_ids.tolist()):
-                out[b].append(t)
+        try:
+            bt.begin(adj, [len(p) + max(1, max_new) for p in prompts])
+            bt.constrain(out)
+            for b, p in enumerate(prompts):
+                us = [rng.random()] if temperature > 0 else None
+                out[b].append(bt.prefill(b, list(p), prm, us))
+            for _ in range(max_new - 1):
+                if temperature > 0:
+                    bt.u.copy_(torch.from_numpy(rng.random(B)))
+                bt.constrain(out)
+                bt.run(prm)
+                for b, t in enumerate(bt.out_ids.tolist()):
+                    out[b].append(t)
+        finally:
+            bt.end()
         return out
+
+    def _paged_batch(self, B, page, pages, rows):
+        """The engine's paged batch of B sequences (kept while its page size fits and its pool is large enough)."""
+        if not isinstance(page, int) or isinstance(page, bool) or page < 1 or page & (page - 1):
+            raise ValueError("the rows of a page must be a power of two")
+        need = sum(-(-n // page) for n in rows)
+        if pages is not None and pages < need:
+            raise ValueError(f"{need} pages of {page} rows are needed, the pool has {pages}")
+        bt = getattr(self, "_pbt", None)
+        if bt is None or bt.B != B or bt.page != page or bt.pages.total < need or pages not in (None, bt.pages.total):
+            self._pbt = None  # the old pool is freed before the new one is made
+            self._pbt = bt = PagedBatch(self, B, page, pages or need)
+        return bt
 
     def _batch(self, B):
         bt = getattr(self, "_bt", None)
@@ -569,7 +605,7 @@ class Batch:
     def __init__(self, eng, B):
         self.eng, self.B = eng, B
         dev, H, KV, HD = eng.device, eng.H, eng.KV, eng.HD
-        self.kv = torch.zeros(B, eng.L, 2, KV, eng.maxt, HD, dtype=torch.bfloat16, device=dev)
+        self._make_cache()
         self.pos = torch.zeros(B, dtype=torch.int64, device=dev)
         self.ids = torch.zeros(B, dtype=torch.int64, device=dev)
         self.out_ids = torch.zeros(B, dtype=torch.int64, device=dev)
@@ -578,23 +614,60 @@ class Batch:
         self.xb, self.hb = f(eng.D), f(eng.D)
         self.qkvb, self.attb, self.gub = f((H + 2 * KV) * HD), f(H * HD), f(2 * eng.FF)
         self.logits = torch.zeros(B, eng.V, device=dev)
-        self.ws = torch.zeros(_lib.lib().aib_attn_batch_workspace(H, KV, HD, eng.maxt, B), dtype=torch.uint8,
-                              device=dev)
         self.sample_ws = sampler.workspace(B, eng.V, dev)
-        self.seq_stride = eng.L * 2 * KV * eng.maxt * HD  # elements between two sequences' caches
         self.graphs = {}
+        self.adj = None
+        self.adj_bufs = {}
 
-    def prefill(self, b, tokens, prm, us):
-        """Prompt of sequence b into its cache (whole-prompt prefill); returns its first token."""
+    def _make_cache(self):
+        eng, B = self.eng, self.B
+        H, KV, HD = eng.H, eng.KV, eng.HD
+        self.kv = torch.zeros(B, eng.L, 2, KV, eng.maxt, HD, dtype=torch.bfloat16, device=eng.device)
+        self.ws = torch.zeros(_lib.lib().aib_attn_batch_workspace(H, KV, HD, eng.maxt, B), dtype=torch.uint8,
+                              device=eng.device)
+        self.seq_stride = eng.L * 2 * KV * eng.maxt * HD  # elements between two sequences' caches
+
+    def begin(self, adj, rows):
+        """Before a batch: adj (an Adjustment or None); rows: cache rows that every sequence will fill."""
+        self.adj = None if adj is None else adj.load(self)
+
+    def end(self):
+        self.adj = None
+
+    def constrain(self, out):
+        """The grammar mask of the next draw, from the tokens so far."""
+        if self.adj is not None and self.adj.next_mask is not None:
+            self.adj.set_mask(self.adj.next_mask(out))
+
+    def _prompt(self, b, tokens):
+        """The layers over the prompt of sequence b, K/V into its cache; the last row is left in eng.xb[0]."""
         eng = self.eng
         own = eng.kv
         eng.kv = self.kv[b]
         try:
-            tok = eng._prefill(tokens, 0, prm, us, False)[0]
+            eng._prompt(tokens, 0)
         finally:
             eng.kv = own
+
+    def prefill(self, b, tokens, prm, us):
+        """Prompt of sequence b into its cache (whole-prompt prefill); returns its first token."""
+        eng = self.eng
+        self._prompt(b, tokens)
+        if prm.temperature > 0:
+            eng.u[0] = us[0]
+        if self.adj is None:
+            eng._pick(1, prm, 1, False)
+        else:
+            tkernels.rmsg(eng.xb[:1], eng.norm, eng.hb[:1], eng.eps)
+            eng._exact(0, 1, 1)
+            self.adj.apply(eng.logits[:1], slice(b, b + 1))
+            sampler.sample_into(eng.logits[:1], eng.out_ids[:1], prm, eng.u[:1] if prm.temperature > 0 else None, B=1,
+                                ws=eng.sample_ws)
+        tok = eng.out_ids[0].item()
         self.pos[b] = len(tokens)
         self.ids[b] = tok
+        if self.adj is not None:
+            self.adj.note(b, len(tokens), tok)
         return tok
 
     def _attn(self, l):
@@ -624,18 +697,22 @@ class Batch:
                 prefill.matrix(self.gub, W["down"], x, add=add, precision=3, silu_input=True, ws=ws)
             eng._reduce(x)
         tkernels.rmsg(x, eng.norm, h, eng.eps)
-        if eng.head8 is not None and prm.temperature <= 0:
+        if eng.head8 is not None and prm.temperature <= 0 and self.adj is None:
             eng.head8.pick(h, B, out=self.out_ids)
         else:
             if eng.tp > 1:
                 raise NotImplementedError("batched decode runs on one GPU (or as replicas)")
             exact_logits(h, eng.head, B, self.logits)
+            if self.adj is not None:
+                self.adj.apply(self.logits, slice(0, B))
             sampler.sample_into(self.logits, self.out_ids, prm, self.u if prm.temperature > 0 else None, None, None,
                                 B=B, ws=self.sample_ws)
-        _lib.call("aib_batch_advance", ptr(self.pos), ptr(self.ids), ptr(self.out_ids), B, stream_ptr())
+        prior = None if self.adj is None else self.adj.prior
+        _lib.call("aib_batch_advance_prior", ptr(self.pos), ptr(self.ids), ptr(self.out_ids), B, ptr(prior),
+                  0 if prior is None else prior.stride(0), 0 if prior is None else prior.shape[1], stream_ptr())
 
     def run(self, prm):
-        key = (prm.temperature, prm.top_k, prm.top_p)
+        key = (prm.temperature, prm.top_k, prm.top_p, None if self.adj is None else self.adj.key)
         if not self.eng.use_graphs:
             self._step(prm)
             return
@@ -655,3 +732,145 @@ class Batch:
         eng = self.eng
         kv = self.B * eng.L * 2 * eng.KV * (ctx + 1) * eng.HD * 2
         return eng.weight_bytes + eng.head_bytes + kv
+
+
+class Adjustment:
+    """What a batch's requests change in their logits before a draw (sampler.adjust): penalties over their recent ids,
+    biases, masks. `load` puts it into buffers that the batch keeps, so that a captured step can be replayed."""
+
+    @staticmethod
+    def of(eng, prompts, repetition, presence, frequency, logit_bias, mask):
+        """None when nothing is to be changed."""
+        B, V = len(prompts), eng.V
+
+        def numbers(x, name):
+            x = [float(v) for v in x] if isinstance(x, (list, tuple)) else [float(x)] * B
+            if len(x) != B:
+                raise ValueError(f"{name}: one number, or one for every prompt")
+            return x
+
+        rep, pres, freq = (numbers(x, n) for x, n in ((repetition, "repetition_penalty"), (presence, "presence_penalty"),
+                                                      (frequency, "frequency_penalty")))
+        if any(not r > 0 for r in rep):
+            raise ValueError("repetition_penalty must be > 0")
+        bias = [dict(d or {}) for d in logit_bias] if logit_bias is not None else [{}] * B
+        if len(bias) != B:
+            raise ValueError("logit_bias: one dictionary (or None) for every prompt")
+        for d in bias:
+            if len(d) > 1024 or any(isinstance(i, bool) or not isinstance(i, int) or not 0 <= i < V for i in d):
+                raise ValueError("logit_bias: at most 1024 ids of the vocabulary a prompt")
+        if mask is not None and not callable(mask):
+            Adjustment._check_mask(mask, B, V)
+        penal = any(r != 1.0 for r in rep) or any(pres) or any(freq)
+        if not penal and not any(bias) and mask is None:
+            return None
+        if eng.tp > 1:
+            raise NotImplementedError("batched adjustment runs on one GPU (or as replicas)")
+        a = Adjustment()
+        a.V, a.lists, a.numbers, a.biases, a.mask_arg = V, prompts if penal else None, (rep, pres, freq), bias, mask
+        return a
+
+    @staticmethod
+    def _check_mask(mask, B, V):
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.int32 or mask.dim() != 2 or \
+                mask.shape[0] not in (1, B) or mask.shape[1] != (V + 31) // 32:
+            raise ValueError("mask must be int32 [B, ceil(V/32)] or one such row")
+
+    def load(self, bt):
+        dev, B, V, bufs = bt.eng.device, bt.B, self.V, bt.adj_bufs
+
+        def buffer(name, *shape, dtype=torch.float32):
+            t = bufs.get((name, *shape))
+            if t is None:
+                t = bufs[(name, *shape)] = torch.zeros(shape, dtype=dtype, device=dev)
+            return t
+
+        self.prior = self.penalties = self.ids = self.bias = self.mask = self.next_mask = None
+        if self.lists is not None:
+            self.prior = buffer("prior", B, sampler.PMAX, dtype=torch.int32)
+            ring = np.full((B, sampler.PMAX), -1, np.int32)
+            for b, p in enumerate(self.lists):
+                for i in range(max(0, len(p) - sampler.PMAX), len(p)):
+                    ring[b, i % sampler.PMAX] = p[i]
+            self.prior.copy_(torch.from_numpy(ring))
+            self.penalties = buffer("penalties", 3, B)
+            self.penalties.copy_(torch.tensor(self.numbers, dtype=torch.float32))
+        n = max(len(d) for d in self.biases)
+        if n:
+            n = 1 << (n - 1).bit_length()  # few sizes, so that few steps are captured
+            self.ids, self.bias = buffer("ids", B, n, dtype=torch.int32), buffer("bias", B, n)
+            ids, val = np.full((B, n), -1, np.int32), np.zeros((B, n), np.float32)
+            for b, d in enumerate(self.biases):
+                ids[b, :len(d)], val[b, :len(d)] = list(d.keys()), list(d.values())
+            self.ids.copy_(torch.from_numpy(ids))
+            self.bias.copy_(torch.from_numpy(val))
+        if self.mask_arg is not None:
+            self.mask = buffer("mask", B, (V + 31) // 32, dtype=torch.int32)
+            if callable(self.mask_arg):
+                self.next_mask = self.mask_arg
+            else:
+                self.set_mask(self.mask_arg)
+        self.key = (self.prior is not None, n, self.mask is not None)
+        return self
+
+    def set_mask(self, mask):
+        self._check_mask(mask, self.mask.shape[0], self.V)
+        self.mask.copy_(mask.expand_as(self.mask))
+
+    def note(self, b, pos, tok):
+        if self.prior is not None:
+            self.prior[b, pos % sampler.PMAX] = tok
+
+    def apply(self, logits, rows):
+        cut = lambda t: None if t is None else t[rows]  # noqa: E731
+        rep, pres, freq = (None,) * 3 if self.penalties is None else (p[rows] for p in self.penalties)
+        sampler.adjust(logits, prior=cut(self.prior), repetition=rep, presence=pres, frequency=freq,
+                       bias_ids=cut(self.ids), bias=cut(self.bias), mask=cut(self.mask))
+
+
+class PagedBatch(Batch):
+    """A batch whose keys and values lie in pages of one pool [L, 2, pages, KV, page, HD]: a sequence costs the pages that
+    it fills. A prompt runs in the engine's own cache and is then copied to its pages; a step appends every sequence's
+    token to its page and attends over the pages (ai_b200.paged)."""
+
+    def __init__(self, eng, B, page, pages):
+        self.page, self.n_pages = page, pages
+        super().__init__(eng, B)
+
+    def _make_cache(self):
+        eng, B = self.eng, self.B
+        dev, H, HD = eng.device, eng.H, eng.HD
+        self.kv = torch.zeros(eng.L, 2, self.n_pages, eng.KV, self.page, HD, dtype=torch.bfloat16, device=dev)
+        self.caches = [paged.Cache(self.kv[l, 0], self.kv[l, 1]) for l in range(eng.L)]
+        self.pages = paged.Pages(self.n_pages, B, -(-eng.maxt // self.page), self.page, dev)
+        self.ws = paged.workspace(B, H, self.caches[0])
+        self.qb = torch.zeros(B, H, HD, device=dev)
+
+    def begin(self, adj, rows):
+        super().begin(adj, rows)
+        for b, n in enumerate(rows):
+            self.pages.grow(b, n)
+
+    def end(self):
+        super().end()
+        for b in range(self.B):
+            self.pages.free(b)
+
+    def _prompt(self, b, tokens):
+        eng, n = self.eng, len(tokens)
+        eng.ctx = []  # the engine's own cache is the workplace
+        eng._prompt(tokens, 0)
+        at = torch.zeros(1, dtype=torch.int64, device=eng.device)
+        cu = torch.tensor([0, n], dtype=torch.int32, device=eng.device)
+        for l, cache in enumerate(self.caches):  # normed and rotated already
+            k, v = (eng.kv[l, i, :, :n].transpose(0, 1) for i in (0, 1))
+            paged.append(cache, self.pages.table[b:b + 1], at, k, v, cu=cu)
+
+    def _attn(self, l):
+        eng, s, B = self.eng, self.eng.small[l], self.B
+        H, KV, HD = eng.H, eng.KV, eng.HD
+        rows = self.qkvb.view(B, H + 2 * KV, HD)
+        paged.append(self.caches[l], self.pages.table, self.pos, rows[:, H:H + KV], rows[:, H + KV:], q=rows[:, :H],
+                     q_out=self.qb, qn=s["qn"], kn=s["kn"], inv=eng.inv, eps=eng.eps)
+        paged.attention(self.qb, self.caches[l], self.pages.table, self.pos, out=self.attb.view(B, H, HD),
+                        scale=eng.scale, ws=self.ws)

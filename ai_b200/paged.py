@@ -37,10 +37,43 @@ class Cache:
             raise ValueError("cache: HD must be 64 or 128 and the rows of a page a power of two")
         if k.stride(3) != 1 or any(s % 8 for s in k.stride()[:3]) or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("cache: rows must be contiguous and 16-byte aligned")
-        self.k, self.v, self.device = k, v, k.device
+        self.k, self.v, self.device, self.index = k, v, k.device, k.get_device()
         self.desc = PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), self.pages, self.page,
                             self.KV, self.HD)
         self.ref = C.byref(self.desc)
+
+
+class Pages:
+    """The pages of a pool and the table of a batch: `table` int32 [B, width] on the device, a sequence's pages in the
+    order of its rows (entries that it does not have are -1)."""
+
+    def __init__(self, pages, B, width, page, device):
+        if pages < 1 or B < 1 or width < 1 or page < 1:
+            raise ValueError("pages, sequences, width and rows per page must be positive")
+        self.total, self.page, self.width = pages, page, width
+        self.left = list(range(pages - 1, -1, -1))
+        self.held = [[] for _ in range(B)]
+        self.table = torch.full((B, width), -1, dtype=torch.int32, device=device)
+
+    def grow(self, b, rows):
+        """Give sequence b the pages that `rows` rows need, all of them or none."""
+        need = -(-rows // self.page) - len(self.held[b])
+        if need <= 0:
+            return
+        if len(self.held[b]) + need > self.width:
+            raise ValueError(f"{rows} rows do not fit a table of {self.width} pages")
+        if need > len(self.left):
+            raise ValueError(f"{need} pages are needed, {len(self.left)} are free")
+        new = [self.left.pop() for _ in range(need)]
+        at = len(self.held[b])
+        self.held[b] += new
+        self.table[b, at:at + need] = torch.tensor(new, dtype=torch.int32, device=self.table.device)
+
+    def free(self, b):
+        """Take sequence b's pages back."""
+        self.left += reversed(self.held[b])
+        self.held[b] = []
+        self.table[b] = -1
 
 
 def _addr(t):
@@ -49,28 +82,33 @@ def _addr(t):
 
 def _check_table(what, cache, table, pos):
     """Returns the batch size and the table's width and row stride."""
-    if pos.dim() != 1 or pos.dtype != torch.int64 or pos.device != cache.device or not pos.is_contiguous():
+    if pos.dim() != 1 or pos.dtype is not torch.int64 or pos.get_device() != cache.index or not pos.is_contiguous():
         raise ValueError(f"{what}: pos must be int64 [B] on the cache's device")
-    B = pos.shape[0]
-    shape, stride = table.shape, table.stride()
-    if len(shape) != 2 or shape[0] != B or shape[1] < 1 or (shape[1] > 1 and stride[1] != 1) or \
-            table.dtype != torch.int32 or table.device != cache.device:
+    B, = pos.shape
+    if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != cache.index:
         raise ValueError(f"{what}: table must be int32 [B, width] on the cache's device")
-    return B, shape[1], stride[0]
+    rows, width = table.shape
+    ld, step = table.stride()
+    if rows != B or width < 1 or (width > 1 and step != 1):
+        raise ValueError(f"{what}: table must be int32 [B, width] on the cache's device")
+    return B, width, ld
 
 
-def _rows(what, t, shape, dtype, device):
+def _rows(what, t, T, heads, cache, dtype):
     """Returns the address and the token and head strides of rows [T, heads, HD]."""
-    stride = t.stride()
-    if t.shape != shape or t.dtype != dtype or t.device != device or stride[2] != 1:
-        raise ValueError(f"append: {what} must be {dtype} {list(shape)} rows on the cache's device")
-    return t.data_ptr(), stride[0], stride[1]
+    if t.dim() == 3 and t.dtype is dtype and t.get_device() == cache.index:
+        n, h, d = t.shape
+        ts, hs, step = t.stride()
+        if n == T and h == heads and d == cache.HD and step == 1:
+            return t.data_ptr(), ts, hs
+    raise ValueError(f"append: {what} must be {dtype} [{T}, {heads}, {cache.HD}] rows on the cache's device")
 
 
-def _vector(what, t, n, dtypes, device):
+def _vector(what, t, n, dtypes, cache):
     if t is None:
         return None
-    if t.dtype not in dtypes or t.shape != (n,) or t.device != device or not t.is_contiguous():
+    if t.dtype not in dtypes or t.dim() != 1 or t.numel() != n or t.get_device() != cache.index or \
+            not t.is_contiguous():
         raise ValueError(f"append: {what} must be {dtypes[0]} [{n}] on the cache's device")
     return t.data_ptr()
 
@@ -78,6 +116,7 @@ def _vector(what, t, n, dtypes, device):
 _NORM = (torch.bfloat16, torch.int16, torch.uint16)
 _F32 = (torch.float32,)
 _I32 = (torch.int32,)
+_NO_ROWS = (None, 0, 0)
 
 
 def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=None, inv=None, eps=1e-6):
@@ -90,22 +129,21 @@ def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=Non
     dt = k.dtype
     if dt not in _DT or k.dim() != 3:
         raise ValueError("append: rows must be fp32 or bf16 [T, heads, HD]")
-    T, KV, HD, dev = k.shape[0], cache.KV, cache.HD, cache.device
+    T, HD = k.shape[0], cache.HD
     if (q is None) != (q_out is None):
         raise ValueError("append: q and q_out go together")
-    kr, vr = _rows("k", k, (T, KV, HD), dt, dev), _rows("v", v, (T, KV, HD), dt, dev)
-    H, qr, qo = 0, (None, 0, 0), (None, 0, 0)
+    H, qr, qo = 0, _NO_ROWS, _NO_ROWS
     if q is not None and q.dim() == 3 and q.shape[1]:
         H = q.shape[1]
-        qr, qo = _rows("q", q, (T, H, HD), dt, dev), _rows("q_out", q_out, (T, H, HD), dt, dev)
-    cu_at = _vector("cu", cu, B + 1, _I32, dev)
+        qr, qo = _rows("q", q, T, H, cache, dt), _rows("q_out", q_out, T, H, cache, dt)
+    kr, vr = _rows("k", k, T, cache.KV, cache, dt), _rows("v", v, T, cache.KV, cache, dt)
     if cu is None and T != B:
         raise ValueError("append: without cu there must be one token per sequence")
-    qn_at, kn_at = _vector("qn", qn, HD, _NORM, dev), _vector("kn", kn, HD, _NORM, dev)
-    inv_at = _vector("inv", inv, HD // 2, _F32, dev)
+    cu_at, inv_at = _vector("cu", cu, B + 1, _I32, cache), _vector("inv", inv, HD // 2, _F32, cache)
+    qn_at, kn_at = _vector("qn", qn, HD, _NORM, cache), _vector("kn", kn, HD, _NORM, cache)
     if T == 0 or B == 0:
         return q_out
-    with _lib.on_device(dev.index) as stream:
+    with _lib.on_device(cache.index) as stream:
         _lib.call("aib_paged_append", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), cu_at, B, T, H, *qr, *kr,
                   *vr, *qo, _DT[dt], qn_at, kn_at, inv_at, eps, stream)
     return q_out
@@ -125,23 +163,24 @@ def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws
     exponentials; scale: default HD ** -0.5; ws: from `workspace` (a fresh one per call when None). A row that attends
     nothing gives zeros and lse -inf. Returns out."""
     B, width, ld = _check_table("attention", cache, table, pos)
-    HD, dev, dt = cache.HD, cache.device, q.dtype
-    shape = q.shape
-    if len(shape) != 3 or shape[0] != B or shape[2] != HD or dt not in _DT or q.device != dev:
+    HD, index, dt = cache.HD, cache.index, q.dtype
+    if q.dim() != 3 or dt not in _DT or q.get_device() != index:
         raise ValueError("attention: q must be fp32 or bf16 [B, H, HD] on the cache's device")
-    H = shape[1]
+    n, H, d = q.shape
+    if n != B or d != HD:
+        raise ValueError("attention: q must be fp32 or bf16 [B, H, HD] on the cache's device")
     if H % cache.KV:
         raise ValueError("attention: the query heads must be a multiple of the key heads")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
-    elif out.shape != shape or out.dtype != dt or out.device != dev:
+        out = torch.empty(q.shape, dtype=dt, device=cache.device)
+    elif out.shape != q.shape or out.dtype is not dt or out.get_device() != index:
         raise ValueError("attention: out must have the shape, type and device of q")
-    q_st, out_st = q.stride(), out.stride()
-    if q_st[2] != 1 or out_st[2] != 1 or (H > 1 and (q_st[1] != HD or out_st[1] != HD)):
+    (q_ld, q_hs, q_step), (out_ld, out_hs, out_step) = q.stride(), out.stride()
+    if q_step != 1 or out_step != 1 or (H > 1 and (q_hs != HD or out_hs != HD)):
         raise ValueError("attention: the heads of a row must be contiguous")
-    if B > 1 and out_st[0] < H * HD:
+    if B > 1 and out_ld < H * HD:
         raise ValueError("attention: the rows of out must be apart")
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (B, H) or lse.device != dev or
+    if lse is not None and (lse.dtype is not torch.float32 or lse.shape != (B, H) or lse.get_device() != index or
                             not lse.is_contiguous()):
         raise ValueError("attention: lse must be fp32 [B, H] on the cache's device")
     if window < 0:
@@ -150,10 +189,10 @@ def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws
         return out
     if ws is None:
         ws = workspace(B, H, cache)
-    elif ws.dtype != torch.uint8 or ws.device != dev or not ws.is_contiguous():
+    elif ws.dtype is not torch.uint8 or ws.get_device() != index or not ws.is_contiguous():
         raise ValueError("attention: ws must come from paged.workspace on the cache's device")
-    with _lib.on_device(dev.index) as stream:
-        _lib.call("aib_paged_attn", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), B, H, q.data_ptr(), q_st[0],
-                  out.data_ptr(), out_st[0], _DT[dt], _addr(lse), window, HD ** -0.5 if scale is None else scale,
+    with _lib.on_device(index) as stream:
+        _lib.call("aib_paged_attn", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), B, H, q.data_ptr(), q_ld,
+                  out.data_ptr(), out_ld, _DT[dt], _addr(lse), window, HD ** -0.5 if scale is None else scale,
                   ws.data_ptr(), ws.numel(), stream)
     return out

@@ -122,3 +122,29 @@ def test_oracle_adjust_by_hand():
     mask = np.array([0b01111], np.uint32).view(np.int32)
     x, _ = opaged.adjust([2.0, -2.0, 1.0, 0.0, 9.0], [0, 1, 1, -1, 7], 2.0, 0.5, 0.25, [2, 2, 9], [1.0, 3.0, 5.0], mask)
     np.testing.assert_array_equal(x, [2.0 / 2 - 0.75, -4.0 - 1.0, 5.0, 0.0, -np.inf])
+
+
+# ------------------------------------------------------------------------------------------------ pages
+def test_pages_are_handed_out_and_come_back():
+    from ai_b200 import paged
+    p = paged.Pages(6, 3, 4, 16, "cpu")
+    p.grow(0, 17)
+    p.grow(2, 48)
+    p.grow(0, 32)  # fits what it has
+    held = p.table.tolist()
+    assert [sum(x >= 0 for x in r) for r in held] == [2, 0, 3]
+    used = [x for r in held for x in r if x >= 0]
+    assert len(set(used)) == 5 and len(p.left) == 1
+    with pytest.raises(ValueError):
+        p.grow(1, 33)  # more than are free: nothing is taken
+    assert len(p.left) == 1 and p.table[1].tolist() == [-1] * 4
+    with pytest.raises(ValueError):
+        p.grow(0, 65)  # wider than the table
+    p.free(2)
+    p.grow(1, 64)
+    assert sum(x >= 0 for x in p.table[1].tolist()) == 4 and not p.left
+    assert p.table[2].tolist() == [-1] * 4
+    assert not set(p.table[1].tolist()) & set(p.table[0, :2].tolist())
+    for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
+        with pytest.raises(ValueError):
+            paged.Pages(*bad, "cpu")
