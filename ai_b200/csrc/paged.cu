@@ -339,15 +339,15 @@ AIB_DEV bool span(const int64_t* pos, int b, int room, long long window, int* lo
 }
 AIB_DEV int units_of(int lo, int hi) { return hi > lo ? (hi - 1) / kBlk - lo / kBlk + 1 : 0; }
 
-// A place in a CTA's run: sequence b, its part s (key head * tiles + tile), whose units are [seg0, seg0 + nblk), counted
-// from the run's first unit (seg0 is negative where the part began in an earlier run).
+// A place in a CTA's run: sequence b, its part (a tile of a key head's query heads), whose units are [seg0, seg0 + nblk),
+// counted from the run's first unit (seg0 is negative where the part began in an earlier run).
 struct Cursor {
-  int seg0, nblk, b, s, lo, hi;
+  int seg0, nblk, b, kvh, tile, lo, hi;
 };
 struct Line {
   const int64_t* pos;
   long long window;
-  int B, room, parts;
+  int B, room, KV, tiles;
 };
 AIB_DEV void enter(Cursor& c, const Line& l) {
   span(l.pos, c.b, l.room, l.window, &c.lo, &c.hi);
@@ -356,8 +356,12 @@ AIB_DEV void enter(Cursor& c, const Line& l) {
 AIB_DEV void seek(Cursor& c, const Line& l, int u) {  // forward to the part that holds unit u
   while (u - c.seg0 >= c.nblk) {
     c.seg0 += c.nblk;
-    if (++c.s == l.parts) {
-      c.s = 0;
+    if (++c.tile == l.tiles) {
+      c.tile = 0;
+      ++c.kvh;
+    }
+    if (c.kvh == l.KV) {
+      c.kvh = 0;
       do {
         if (++c.b >= l.B) {  // not reached while pos stays as it was
           c.b = l.B - 1;
@@ -389,16 +393,20 @@ AIB_DEV void write_out(E* out, float* lse, float M, float L, float4 a, int d, bo
   if (lse && d == 0) *lse = lse_of(M, L);
 }
 
-struct Owner {  // what a state in shared memory belongs to (b < 0: there is none)
-  int b, s, seg0, nblk;
+struct Owner {  // what a state in shared memory belongs to: heads h0 .. h0 + nh - 1 of b (b < 0: there is none)
+  int b, h0, nh, seg0, nblk;
 };
+// a / b for a that is nearly always below 2^31 (a 64-bit division takes most of a microsecond)
+AIB_DEV long long quotient(long long a, int b) {
+  return a >> 31 ? a / b : static_cast<unsigned>(a) / static_cast<unsigned>(b);
+}
 template <int HD>
 struct Shared {
   uint64_t full[Lay<HD>::kWarps][kTiles];
   long long wtot[Lay<HD>::kWarps], base;
   Owner own[2 * Lay<HD>::kWarps];  // the warps' first states (parts that began before the piece) and last states
   float M[GT], L[GT];
-  int b, abort, last[2];
+  int b, abort, last[2], c0[2], np[2];
 };
 
 template <int HD, typename E>
@@ -418,7 +426,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x, grid = gridDim.x;
   const int G = H / KV, tiles = (G + GT - 1) / GT;
-  const Line line{pos, window, B, room, KV * tiles};
+  const Line line{pos, window, B, room, KV, tiles};
+  const int parts = KV * tiles;
   if (lane < kTiles) mbar_init(&sh.full[warp][lane], 1);
   if (lane < 2) sh.own[2 * warp + lane].b = -1;
   if (threadIdx.x == 0) {
@@ -439,7 +448,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     if (!span(pos, b, room, window, &lo, &hi) && cta == 0) set_status(AIB_DEV_BAD_POS);
     mine += units_of(lo, hi);
   }
-  mine *= line.parts;
+  mine *= parts;
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -454,16 +463,16 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     if (w < warp) before += sh.wtot[w];
     total += sh.wtot[w];
   }
-  const long long per = max(static_cast<long long>(Y::kMinRun), (total + grid - 1) / grid);
-  const long long u0 = cta * per;
-  const int n = static_cast<int>(max(0LL, min(total - u0, per)));
+  const int per = static_cast<int>(max(static_cast<long long>(Y::kMinRun), quotient(total + grid - 1, grid)));
+  const long long u0 = static_cast<long long>(cta) * per;
+  const int n = static_cast<int>(max(0LL, min(total - u0, static_cast<long long>(per))));
   if (n > 0) {
     long long base = before + incl - mine;
     if (u0 >= base && u0 < base + mine) {
       for (int b = b_lo; b < b_hi; ++b) {
         int lo, hi;
         span(pos, b, room, window, &lo, &hi);
-        const long long m = static_cast<long long>(units_of(lo, hi)) * line.parts;
+        const long long m = static_cast<long long>(units_of(lo, hi)) * parts;
         if (u0 < base + m) {
           sh.b = b;
           sh.base = base;
@@ -482,8 +491,10 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     Cursor C;
     C.b = sh.b;
     enter(C, line);
-    C.s = static_cast<int>((u0 - sh.base) / C.nblk);
-    C.seg0 = -static_cast<int>((u0 - sh.base) % C.nblk);
+    const int part = static_cast<int>(quotient(u0 - sh.base, C.nblk));
+    C.seg0 = -static_cast<int>(u0 - sh.base - static_cast<long long>(part) * C.nblk);
+    C.kvh = part / tiles;
+    C.tile = part - C.kvh * tiles;
     seek(C, line, beg);
 
     // copies: a lane stands for a box of a unit
@@ -500,7 +511,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
         seek(P, line, u + bu);
         const int j0 = (P.lo & ~(kBlk - 1)) + (u + bu - P.seg0) * kBlk, a = j0 + bx * box;
         const int r0 = max(a, P.lo) - j0, r1 = min(a + box, P.hi) - j0;  // within the unit
-        k.kvh = P.s / tiles;
+        k.kvh = P.kvh;
         k.row = a & ((1 << page_shift) - 1);
         if (r0 < r1) {
           k.rows = (0xffffffffu >> (32 - (r1 - r0))) << r0;
@@ -514,6 +525,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     Look now{-1, 0, 0, 0}, next = look_up(beg);
     uint32_t mask = 0, bytes = 0;       // of the lane's unit
     int at = batch, iu = beg, is = 0;   // place in the batch of the unit whose copies start next, that unit, its tile
+    int started = 0, landed = 0;        // copies of the warp
+    const bool withhold = g_aib_withhold_copies != 0;
     // starts the copies of unit iu's K (and returns the unit's attended rows) or V
     auto start = [&](bool v) {
       if (!v && at == batch) {
@@ -532,11 +545,13 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
         next = look_up(iu + batch);
       }
       uint64_t* bar = &sh.full[warp][is];
+      if (withhold) return 0u;  // test knob 2: the tile never fills
       if (lane == at * nbox) mbar_arrive_expect_tx(bar, bytes);
       __syncwarp();
       if (bu == at && now.rows)
         tma_load<HD>(tile0 + is * Y::kTile + bx * box * HD * 2, v ? &vmap : &kmap, bar, now.row, now.kvh, now.id);
       const uint32_t vm = __shfl_sync(0xffffffffu, mask, at * nbox);
+      ++started;
       is = is == kTiles - 1 ? 0 : is + 1;
       if (v) {
         ++at;
@@ -572,6 +587,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     auto wait = [&]() {
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.full[warp][cs], ph, AIB_DEV_TIMEOUT_FULL));
       const int tile = cs;
+      if (ok) ++landed;
       if (++cs == kTiles) {
         cs = 0;
         ph ^= 1;
@@ -579,7 +595,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
       return tile;
     };
     while (true) {
-      const int h0 = (C.s / tiles) * G + (C.s % tiles) * GT, nh = min(GT, G - (C.s % tiles) * GT);
+      const int h0 = C.kvh * G + C.tile * GT, nh = min(GT, G - C.tile * GT);
       const int stop = min(end, C.seg0 + C.nblk);
       float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
       float acc[NT][4];
@@ -722,44 +738,41 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
             dst[HD + 1] = hh ? l1 : l0;
           }
         }
-        if (lane == 0) sh.own[2 * warp + (ended ? 0 : 1)] = Owner{C.b, C.s, C.seg0, C.nblk};
+        if (lane == 0) sh.own[2 * warp + (ended ? 0 : 1)] = Owner{C.b, h0, nh, C.seg0, C.nblk};
       }
       if (u >= end) break;
       seek(C, line, u);
     }
     if (!ok) {  // a wait ran out: the copies that are still on their way must land before the CTA ends
       sh.abort = 1;
-      for (int k = 0; k < kTiles; ++k) {
-        mbar_wait(&sh.full[warp][cs], ph, AIB_DEV_TIMEOUT_FULL);
-        if (++cs == kTiles) {
-          cs = 0;
-          ph ^= 1;
+      for (int k = landed; k < started; ++k)
+        for (uint32_t i = 0; i < kSpinLimit && !mbar_try_wait(&sh.full[warp][k % kTiles], k / kTiles & 1); ++i) {
         }
-      }
     }
   }
   __syncthreads();
 
   // ---- parts that cross warps: their states, neighbours among the 2 NW places, are joined in order
-  Owner o{-1, 0, 0, 0};
+  Owner o{-1, 0, 0, 0, 0};
   if (lane < 2 * NW) o = sh.own[lane];
   const uint32_t there = sh.abort ? 0 : __ballot_sync(0xffffffffu, o.b >= 0);
   if (there) {
     const uint32_t below = there & ((1u << lane) - 1);
     const int prev = below ? 31 - __clz(below) : 0;
-    const int pb = __shfl_sync(0xffffffffu, o.b, prev), ps = __shfl_sync(0xffffffffu, o.s, prev);
-    const uint32_t heads = __ballot_sync(0xffffffffu, o.b >= 0 && (!below || pb != o.b || ps != o.s));
-    const int ng = __popc(heads), items = min(G, GT) * (HD / 4);
-    for (int i = threadIdx.x; i < ng * items; i += Y::kThreads) {
+    const int pb = __shfl_sync(0xffffffffu, o.b, prev), ph0 = __shfl_sync(0xffffffffu, o.h0, prev);
+    const uint32_t heads = __ballot_sync(0xffffffffu, o.b >= 0 && (!below || pb != o.b || ph0 != o.h0));
+    // items of four dimensions: as many heads a group as the next power of two, HD / 4 items a head
+    const int ng = __popc(heads), head_bits = 32 - __clz(min(G, GT) - 1);
+    constexpr int kItemBits = HD == 128 ? 5 : 4;
+    for (int i = threadIdx.x; i < ng << (head_bits + kItemBits); i += Y::kThreads) {
       uint32_t rest = heads;
-      for (int k = i / items; k > 0; --k) rest &= rest - 1;
+      for (int k = i >> (head_bits + kItemBits); k > 0; --k) rest &= rest - 1;
       const int lo = __ffs(rest) - 1;
       rest &= rest - 1;
       const uint32_t set = there & (0xffffffffu << lo) & (rest ? (1u << (__ffs(rest) - 1)) - 1 : 0xffffffffu);
       const Owner w = sh.own[lo];
-      const int h = i % items / (HD / 4), d = i % (HD / 4) * 4;
-      const int h0 = (w.s / tiles) * G + (w.s % tiles) * GT;
-      if (h >= min(GT, G - (w.s % tiles) * GT)) continue;
+      const int h = i >> kItemBits & ((1 << head_bits) - 1), d = i % (HD / 4) * 4;
+      if (h >= w.nh) continue;
       auto state = [&](int k) {
         return (k & 1 ? reinterpret_cast<const float*>(ring + (k >> 1) * kTiles * Y::kTile) : first + (k >> 1) * Y::kPart) +
                h * W;
@@ -790,8 +803,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
         L += e * ml[k].y;
       }
       if (w.seg0 >= 0 && w.seg0 + w.nblk <= n) {
-        write_out(out + w.b * out_ld + static_cast<long long>(h0 + h) * HD,
-                  lse ? lse + static_cast<long long>(w.b) * H + h0 + h : nullptr, M, L, a, d, vec);
+        write_out(out + w.b * out_ld + static_cast<long long>(w.h0 + h) * HD,
+                  lse ? lse + static_cast<long long>(w.b) * H + w.h0 + h : nullptr, M, L, a, d, vec);
       } else {
         float* part = parts_ws + static_cast<long long>(2 * cta + (w.seg0 >= 0 ? 1 : 0)) * Y::kPart + h * W;
         *reinterpret_cast<float4*>(part + d) = a;
@@ -802,7 +815,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     // ---- parts that cross CTAs, the run's first and last at most: the last CTA to finish joins the partial states
     const int e0 = __ffs(there) - 1, e1 = 31 - __clz(there);
     const Owner ends[2] = {sh.own[e0], sh.own[e1]};
-    const bool one = ends[0].b == ends[1].b && ends[0].s == ends[1].s;
+    const bool one = ends[0].b == ends[1].b && ends[0].h0 == ends[1].h0;
     bool cross[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) cross[x] = (ends[x].seg0 < 0 || ends[x].seg0 + ends[x].nblk > n) && !(x && one);
@@ -813,7 +826,10 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
         const Owner w = ends[threadIdx.x];
         bool last = false;
         if (cross[threadIdx.x]) {
-          const int c0 = static_cast<int>((u0 + w.seg0) / per), c1 = static_cast<int>((u0 + w.seg0 + w.nblk - 1) / per);
+          // the CTAs before this one and after it that have units of the part
+          const int c0 = cta - (w.seg0 < 0 ? (per - 1 - w.seg0) / per : 0), c1 = cta + (w.seg0 + w.nblk - 1) / per;
+          sh.c0[threadIdx.x] = c0;
+          sh.np[threadIdx.x] = c1 - c0 + 1;
           last = atomicAdd(&cnt[c0], 1) == c1 - c0;
           if (last) {
             cnt[c0] = 0;
@@ -829,13 +845,13 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
       for (int x = 0; x < 2; ++x) {
         if (!sh.last[x]) continue;
         const Owner w = ends[x];
-        const int c0 = static_cast<int>((u0 + w.seg0) / per), np = static_cast<int>((u0 + w.seg0 + w.nblk - 1) / per) - c0 + 1;
-        const int h0 = (w.s / tiles) * G + (w.s % tiles) * GT, nh = min(GT, G - (w.s % tiles) * GT);
+        const int c0 = sh.c0[x], np = sh.np[x], nh = w.nh;
         auto part_of = [&](int k) {  // the k-th CTA's state
           return parts_ws + static_cast<long long>(2 * (c0 + k) + (k == 0)) * Y::kPart;
         };
-        for (int i = threadIdx.x; i < nh * np; i += Y::kThreads) {
-          const int h = i % nh, k = i / nh;
+        for (int i = threadIdx.x; i < np << head_bits; i += Y::kThreads) {
+          const int h = i & ((1 << head_bits) - 1), k = i >> head_bits;
+          if (h >= nh) continue;
           const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(k) + h * W + HD));
           pm[h * kMaxGrid + k] = ml.x;
           pl[h * kMaxGrid + k] = ml.y;
@@ -886,8 +902,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
           a.z += __shfl_xor_sync(0xffffffffu, a.z, 16);
           a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
           if (half == 0)
-            write_out(out + w.b * out_ld + static_cast<long long>(h0 + h) * HD,
-                      lse ? lse + static_cast<long long>(w.b) * H + h0 + h : nullptr, sh.M[h], sh.L[h], a, d, vec);
+            write_out(out + w.b * out_ld + static_cast<long long>(w.h0 + h) * HD,
+                      lse ? lse + static_cast<long long>(w.b) * H + w.h0 + h : nullptr, sh.M[h], sh.L[h], a, d, vec);
         }
         if (!weighed) weigh();
         __syncthreads();  // the weights are rewritten next
@@ -913,9 +929,11 @@ static int check_kv(const char* what, const aib_paged_kv* c, Kv* o) {
   if (c->page <= 0 || (c->page & (c->page - 1)))
     return fail(AIB_EINVAL, "%s: rows per page must be a power of two (%d)", what, c->page);
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) ||
-      ((c->page_stride | c->head_stride | c->row_stride) & 7) || c->page_stride < 0 || c->head_stride < 0 ||
-      c->row_stride < 0)
-    return fail(AIB_EINVAL, "%s: cache rows must start on 16-byte boundaries, strides must not be negative", what);
+      ((c->page_stride | c->head_stride | c->row_stride) & 7))
+    return fail(AIB_EINVAL, "%s: cache rows must start on 16-byte boundaries", what);
+  if ((c->pages > 1 && c->page_stride < c->HD) || (c->KV > 1 && c->head_stride < c->HD) ||
+      (c->page > 1 && c->row_stride < c->HD))
+    return fail(AIB_EINVAL, "%s: cache rows overlap", what);
   *o = Kv{c->k, c->v, c->page_stride, c->head_stride, c->row_stride, c->pages, c->KV, __builtin_ctz(c->page)};
   return AIB_OK;
 }

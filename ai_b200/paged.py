@@ -37,6 +37,8 @@ class Cache:
             raise ValueError("cache: HD must be 64 or 128 and the rows of a page a power of two")
         if k.stride(3) != 1 or any(s % 8 for s in k.stride()[:3]) or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("cache: rows must be contiguous and 16-byte aligned")
+        if any(n > 1 and s < self.HD for n, s in zip(k.shape[:3], k.stride()[:3])):
+            raise ValueError("cache: rows must not overlap")
         self.k, self.v, self.device, self.index = k, v, k.device, k.get_device()
         self.desc = PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), self.pages, self.page,
                             self.KV, self.HD)
@@ -151,14 +153,15 @@ def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=Non
 
 def workspace(B, H, cache):
     """Scratch of `attention` for up to B sequences and H query heads (zero-filled once; calls leave it reusable). Calls
-    that may overlap on the GPU need separate ones."""
+    that may overlap on the GPU need separate ones. After a device status of 101 (a wait that ran out) it has to be
+    zeroed again."""
     n = _lib.lib().aib_paged_attn_workspace(B, H, cache.KV, cache.HD)
     return torch.zeros(max(n, 16), dtype=torch.uint8, device=cache.device)
 
 
 def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws=None):
-    """Attention of one new token per sequence: q [B, H, HD] (fp32 or bf16, heads contiguous; normed and rotated), its
-    own key and value already in the cache at pos[b]. Attends positions 0 .. pos[b], or with a window the last `window`
+    """Attention of one new token per sequence (at most 4096): q [B, H, HD] (fp32 or bf16, heads contiguous; normed and
+    rotated), its own key and value already in the cache at pos[b]. Attends positions 0 .. pos[b], or with a window the last `window`
     of them. out: [B, H, HD] like q (allocated when None); lse: optional fp32 [B, H], the log of the summed
     exponentials; scale: default HD ** -0.5; ws: from `workspace` (a fresh one per call when None). A row that attends
     nothing gives zeros and lse -inf. Returns out."""

@@ -71,8 +71,9 @@ void aib_set_pdl(int enabled);
 int aib_status_read(int* out, int clear);
 /* Test knobs of the current device (synchronous; no reference counterpart), so that tests can make a bounded wait
  * run out without any fault: knob 1 = spin limit of every bounded wait (polls; 0 restores the default, 2^22 polls,
- * far longer than any legitimate wait), knob 2 = 1 makes the wide T = 1 GEMV's producer withhold its copies (its stages
- * never fill, its consumers give up after the spin limit and record AIB_DEV_TIMEOUT_FULL), knob 3 = how many
+ * far longer than any legitimate wait), knob 2 = 1 makes the wide T = 1 GEMV's producer and the paged attention
+ * withhold their copies (the stages never fill, those who wait give up after the spin limit and record
+ * AIB_DEV_TIMEOUT_FULL), knob 3 = how many
  * thread-block cluster sizes (16, then 8 CTAs) the decode attention tries for its cluster merge before the
  * ticket merge (default 0: ticket merge only; its feasibility query is not allowed inside a graph capture),
  * knob 4 = the T = 1 GEMV kernel: 3 (default) the tensor-core wide-stage kernel, two CTAs per SM where the
@@ -260,8 +261,8 @@ int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t ta
  * rows at q_ld) attends positions max(0, pos[b] - window + 1) .. pos[b] (window 0: 0 .. pos[b]); out [B, H, HD] (rows
  * at out_ld), lse fp32 [B, H] or NULL = log of the sum of exp(scale * q.k). A row that attends nothing gives zeros and
  * lse -inf. dtype of q and out: 0 fp32 (products and sums as accurate as fp32), 1 bf16. H a multiple of KV.
- * ws: aib_paged_attn_workspace(...) bytes, 16-byte aligned, zero-filled once (left zeroed where it must be); calls that
- * may overlap on the GPU need separate ones. B <= 4096. */
+ * ws: aib_paged_attn_workspace(...) bytes, 16-byte aligned, zero-filled once (left zeroed where it must be, unless a
+ * wait ran out: AIB_DEV_TIMEOUT_FULL); calls that may overlap on the GPU need separate ones. B <= 4096. */
 size_t aib_paged_attn_workspace(int B, int H, int KV, int HD);
 int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t table_ld, int max_pages,
                    const int64_t* pos, int B, int H, const void* q, int64_t q_ld, void* out, int64_t out_ld, int dtype, float* lse,

@@ -385,6 +385,144 @@ def test_step_captured_on_another_stream(mod):
     assert torch.equal(caches[0].k, caches[1].k) and lib.status() == 0
 
 
+def test_attention_wait_runs_out_reports_status_and_recovers(mod):
+    """Copies that never come: every wait gives up, the status says so, and the context stays usable."""
+    paged, _, lib = mod
+    g = gen(21)
+    pos, page = [700, 5, 90], 16
+    c = make_cache(paged, 60, 2, page, 128, g)
+    table = make_table([p + 1 for p in pos], page, 60, g)
+    q = torch.randn(3, 8, 128, generator=g, device="cuda")
+    ws = paged.workspace(3, 8, c)
+    lib.call("aib_debug_knob", 1, 4096)
+    lib.call("aib_debug_knob", 2, 1)
+    try:
+        run_attention(paged, c, q, table, pos, 0, ws=ws)
+        torch.cuda.synchronize()
+        st = lib.status(clear=True)
+    finally:
+        lib.call("aib_debug_knob", 2, 0)
+        lib.call("aib_debug_knob", 1, 0)
+    assert st == 101
+    ws.zero_()
+    out, lse = run_attention(paged, c, q, table, pos, 0, ws=ws)
+    check_attention(c, q, table, pos, 0, 128 ** -0.5, out, lse)
+    assert lib.status() == 0
+
+
+@pytest.mark.parametrize("HD,dtype", [(128, "f32"), (64, "bf16")])
+def test_attention_batches_of_every_size(mod, HD, dtype):
+    """From one row to the largest batch, with rows of one token, unused rows and a shared table row."""
+    paged, _, lib = mod
+    g = gen(22)
+    page, KV, H = 4, 1, 2
+    c = make_cache(paged, 512, KV, page, HD, g)
+    for B in (1, 2, 257, 4096):
+        r = np.random.default_rng(B)
+        pos = [int(p) for p in r.choice([-1, 0, 1, 3, 4, 30, 31, 32, 33, 70], B)]
+        table = torch.randint(0, 512, (1, 18), generator=g, device="cuda", dtype=torch.int32).expand(B, 18)
+        q = torch.randn(B, H, HD, generator=g, device="cuda").to(DT[dtype])
+        out, lse = run_attention(paged, c, q, table, pos, 0)
+        check_attention(c, q, table, pos, 0, HD ** -0.5, out, lse)
+    assert lib.status() == 0
+
+
+def test_attention_rows_apart_and_odd(mod):
+    """q and out as cuts of wider rows, on addresses that allow no wide access; what lies between stays."""
+    paged, _, lib = mod
+    g = gen(23)
+    pos, H, HD, page = [40, 300], 6, 64, 32
+    c = make_cache(paged, 16, 2, page, HD, g, "rows")
+    table = make_table([p + 1 for p in pos], page, 16, g)
+    for dt in DT.values():
+        wide = torch.randn(2, H * HD + 11, generator=g, device="cuda").to(dt)
+        res = torch.full((2, H * HD + 7), 9.0, device="cuda", dtype=dt)
+        q, out = wide[:, 3:3 + H * HD].view(2, H, HD), res[:, 5:5 + H * HD].view(2, H, HD)
+        paged.attention(q, c, table, torch.tensor(pos, device="cuda"), out=out)
+        check_attention(c, q.contiguous(), table, pos, 0, HD ** -0.5, out, None)
+        assert (res[:, :5] == 9).all() and (res[:, 5 + H * HD:] == 9).all()
+    assert lib.status() == 0
+
+
+def test_graphs_that_share_a_workspace(mod):
+    """Two captured calls with one workspace, replayed in turn in one stream, and an eager call between."""
+    paged, _, lib = mod
+    g = gen(24)
+    c = make_cache(paged, 400, 2, 16, 128, g)
+    ws = paged.workspace(8, 8, c)
+    made = []
+    for pos in ([3000], [700, 20, 1500]):
+        table = make_table([p + 1 for p in pos], 16, 400, g)
+        q = torch.randn(len(pos), 8, 128, generator=g, device="cuda")
+        p = torch.tensor(pos, device="cuda")
+        want = paged.attention(q, c, table, p, ws=ws).clone()
+        out = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            paged.attention(q, c, table, p, out=out, ws=ws)
+        made.append((graph, out, want, (q, c, table, p)))
+    for _ in range(3):
+        for graph, out, want, args in made:
+            out.zero_()
+            graph.replay()
+            assert torch.equal(out, want)
+            assert torch.equal(paged.attention(*args, ws=ws), want)
+    assert lib.status() == 0
+
+
+def test_python_refusals(mod):
+    """Shapes, types, strides and devices that do not fit raise ValueError before anything is launched."""
+    paged, sampler, lib = mod
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
+    b, i32, i64 = torch.bfloat16, torch.int32, torch.int64
+    kv = lambda *s: (z(*s, dtype=b), z(*s, dtype=b))  # noqa: E731
+    for k, v in (kv(2, 2, 16, 96), kv(2, 2, 12, 64), (z(2, 2, 16, 64), z(2, 2, 16, 64)),
+                 (kv(2, 2, 16, 64)[0], kv(2, 2, 8, 64)[0]), (kv(2, 2, 16, 65)[0][..., 1:],) * 2,
+                 (kv(2, 2, 16, 128)[0][..., ::2],) * 2, (kv(1, 1, 16, 64)[0].expand(2, 2, 16, 64),) * 2,
+                 (kv(2, 2, 16, 64)[0], kv(2, 2, 16, 64)[0].cpu())):
+        with pytest.raises(ValueError):
+            paged.Cache(k, v)
+    c = paged.Cache(*kv(4, 2, 16, 64))
+    t, p, k = z(3, 2, dtype=i32), z(3, dtype=i64), z(3, 2, 64)
+    good = dict(cache=c, table=t, pos=p, k=k, v=k, q=z(3, 4, 64), q_out=z(3, 4, 64))
+    for bad in (dict(table=z(2, 2, dtype=i32)), dict(table=z(3, 2, dtype=i64)), dict(table=t.cpu()),
+                dict(table=z(3, 4, dtype=i32)[:, ::2]), dict(pos=z(3)), dict(pos=z(6, dtype=i64)[::2]), dict(pos=p.cpu()),
+                dict(k=k.half()), dict(k=k.to(b)), dict(k=z(3, 2, 128)[..., ::2]), dict(v=z(3, 1, 64)),
+                dict(q=z(3, 4, 128)), dict(q_out=None), dict(q_out=z(3, 4, 64).to(b)), dict(q=z(3, 4, 64).cpu()),
+                dict(cu=z(3, dtype=i32)), dict(cu=z(4, dtype=i64)), dict(inv=z(64)), dict(inv=z(32).to(b)),
+                dict(qn=z(64)), dict(kn=z(32, dtype=b)), dict(k=z(2, 2, 64), v=z(2, 2, 64), q=None, q_out=None)):
+        with pytest.raises(ValueError):
+            paged.append(**{**good, **bad})
+    good = dict(q=z(3, 4, 64), cache=c, table=t, pos=p)
+    for bad in (dict(q=z(3, 3, 64)), dict(q=z(2, 4, 64)), dict(q=z(3, 4, 64).half()), dict(q=z(3, 4, 64).cpu()),
+                dict(q=z(3, 4, 128)), dict(q=z(3, 8, 64)[:, ::2]), dict(out=z(3, 4, 64).to(b)), dict(out=z(3, 2, 64)),
+                dict(out=z(1, 4, 64).expand(3, 4, 64)), dict(lse=z(3)), dict(lse=z(4, 3).t()), dict(window=-1),
+                dict(ws=z(1 << 20)), dict(ws=z(1, dtype=torch.uint8).cpu())):
+        with pytest.raises(ValueError):
+            paged.attention(**{**good, **bad})
+    with pytest.raises(RuntimeError):
+        paged.attention(**good, ws=z(64, dtype=torch.uint8))
+    x, W = z(3, 70), z(3, 3, dtype=i32)
+    wide = z(3, 80)
+    for bad in (dict(logits=x[0]), dict(logits=x.half()), dict(logits=x.double()), dict(logits=z(3, 140)[:, ::2]),
+                dict(out=z(3, 71)), dict(out=x.to(b)), dict(logits=wide[:, :70], out=wide[:, 10:]),
+                dict(out=z(1, 70).expand(3, 70)), dict(prior=z(2, 5, dtype=i32)), dict(prior=z(3, 5, dtype=i64)),
+                dict(prior=z(3, 5, dtype=i32).cpu()), dict(mask=z(3, 2, dtype=i32)), dict(mask=z(3, 6, dtype=i32)[:, ::2]),
+                dict(bias_ids=W), dict(bias=z(3, 3)), dict(bias_ids=W, bias=z(3, 4)), dict(repetition=z(2)),
+                dict(presence=z(3).double()), dict(frequency=z(6)[::2])):
+        with pytest.raises(ValueError):
+            sampler.adjust(**{"logits": x, **bad})
+    with pytest.raises(RuntimeError):
+        sampler.adjust(x, prior=z(3, 32768, dtype=i32), repetition=z(3))
+    with pytest.raises(RuntimeError):
+        sampler.adjust(x, bias_ids=z(3, 1025, dtype=i32), bias=z(3, 1025))
+    # nothing to do: no tokens, no rows
+    assert paged.append(c, z(0, 1, dtype=i32), z(0, dtype=i64), z(0, 2, 64), z(0, 2, 64)) is None
+    assert paged.attention(z(0, 4, 64), c, z(0, 1, dtype=i32), z(0, dtype=i64)).shape == (0, 4, 64)
+    assert sampler.adjust(z(0, 70)).shape == (0, 70) and sampler.adjust(z(3, 0)).shape == (3, 0)
+    assert lib.status() == 0
+
+
 # ---------------------------------------------------------------------------------------------- adjust
 ADJUST = [  # B, V, prior ids, biases, mask, logits row stride beyond V, out row stride beyond V
     (1, 1, 0, 0, False, 0, 0),

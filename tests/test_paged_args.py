@@ -45,7 +45,7 @@ def attn(L, c=None, **kw):
 
 BAD_CACHE = [(dict(k=None), -1), (dict(v=None), -1), (dict(pages=0), -1), (dict(KV=0), -1), (dict(HD=96), -4),
              (dict(page=0), -1), (dict(page=24), -1), (dict(k=(1 << 20) + 8), -1), (dict(row_stride=132), -1),
-             (dict(page_stride=-4096), -1)]
+             (dict(page_stride=-4096), -1), (dict(head_stride=64), -1), (dict(row_stride=0), -1)]
 
 
 @pytest.mark.parametrize("bad,code", BAD_CACHE)
