@@ -6,7 +6,7 @@
 // counts the row's prior ids that fall into the slice in shared memory (15 bits a token, the 16th says that the token has
 // a bias). After the copy every entry of the lists that falls into the slice writes its token's adjusted logit, computed
 // from the raw one; entries of the same token write the same value. In place they first read, then write, and clear the
-// counts of what they have written. Bound by bytes; a slice is as long as the grid allows (five CTAs an SM), since every
+// counts of what they have written. Bound by bytes; a slice is as long as the grid allows (four CTAs an SM), since every
 // slice reads the whole of the row's lists.
 // Slices are cut in a shifted index u = v + sh, where sh is the row's distance from a 16-byte boundary in elements, so
 // that vector accesses are aligned whatever the row's start.
@@ -55,8 +55,22 @@ AIB_DEV void mask_out(uint4& x, uint32_t bits, uint16_t) {
   x = make_uint4(mask_pair(x.x, bits), mask_pair(x.y, bits >> 2), mask_pair(x.z, bits >> 4), mask_pair(x.w, bits >> 6));
 }
 
+// Loads that the compiler may not put off until their values are used (the lists' work lies between): the slice's data,
+// read once, and the mask's words, which neighbours read too. 256 rows of 151669 bf16
+// with a mask alone: 32 us with plain loads, 26 us with these.
+AIB_DEV uint4 load_now(const uint4* p) {
+  uint4 x;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p));
+  return x;
+}
+AIB_DEV uint32_t load_now(const uint32_t* p) {
+  uint32_t x;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
+}
+
 template <typename E, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1280 / kThreads)
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
     adjust_kernel(const E* logits, long long ld, E* out, long long out_ld, int V, const int32_t* __restrict__ prior,
                   long long prior_ld, int n_prior, const float* __restrict__ rep, const float* __restrict__ pres,
                   const float* __restrict__ freq, const int32_t* __restrict__ bias_ids, long long ids_ld,
@@ -96,10 +110,10 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
 #pragma unroll
     for (int j = 0; j < kDeep; ++j) {
       if (whole(k + j * kStep)) {
-        x[j] = __ldcs(src + (k - at) / N + j * kThreads);
+        x[j] = load_now(src + (k - at) / N + j * kThreads);
         if (mrow) {
-          lo[j] = words[(k - at) / 32 + j * (kStep / 32)];
-          if (two) hi[j] = words[(k - at) / 32 + j * (kStep / 32) + 1];
+          lo[j] = load_now(words + (k - at) / 32 + j * (kStep / 32));
+          if (two) hi[j] = load_now(words + (k - at) / 32 + j * (kStep / 32) + 1);
         }
       }
     }
@@ -107,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
   load(at);
 
   // ---- counts of the slice's tokens. The lists' first entries are on their way before the table is clear.
-  constexpr int kItems = 4;  // entries of a thread at once: a group of four neighbours
+  constexpr int kItems = kThreads == 512 ? 8 : 4;  // entries of a thread at once: groups of four neighbours
   const int32_t* pr = prior + b * prior_ld;
   const int32_t* ids = bias_ids + b * ids_ld;
   const bool quad = !(reinterpret_cast<uintptr_t>(pr) & 15);
@@ -205,20 +219,33 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
     }
     return z;
   };
-  for (int i0 = 0; i0 < groups; i0 += kThreads * kItems / 4) {
-    if (groups > kThreads * kItems / 4) entries(i0);
-    uint32_t c[kItems];
-    float z[kItems];
+  // A round takes a thread's groups of prior ids and two biases: all that they read is on its way before anything is
+  // written (in place nothing may be written before everything is read).
+  constexpr int kBiases = 2;
+  constexpr int kGroups = kItems / 4 * kThreads;  // groups of a round
+  for (int round = 0; round * kGroups < groups || round * kThreads * kBiases < n_bias; ++round) {
+    if (groups > kGroups) entries(round * kGroups);  // (a single round's are still there from the counting)
+    uint32_t c[kItems], cb[kBiases];
+    float z[kItems], zb[kBiases];
+    int tb[kBiases];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
-      c[i] = count_of(id[i]);
+      c[i] = round * kGroups < groups ? count_of(id[i]) : 0;
       if (c[i] & kBiased) c[i] = 0;  // the biases' entries see to it
     }
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      z[i] = c[i] ? to_f(logits[id[i]]) : 0.0f;
-      if (c[i] && !allowed(id[i])) c[i] = 0;
+    for (int j = 0; j < kBiases; ++j) {
+      const int i = (round * kBiases + j) * kThreads + threadIdx.x;
+      tb[j] = i < n_bias ? bid[i] : -1;
+      cb[j] = count_of(tb[j]);  // 0 for a token that an earlier round has written
     }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) z[i] = c[i] ? to_f(logits[id[i]]) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kBiases; ++j) zb[j] = cb[j] ? to_f(logits[tb[j]]) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (c[i] && !allowed(id[i])) c[i] = 0;
     if (in_place) __syncthreads();
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
@@ -227,26 +254,22 @@ __global__ void __launch_bounds__(kThreads, 1280 / kThreads)
         if (in_place) reinterpret_cast<uint16_t*>(cnt)[id[i] - base] = 0;
       }
     }
-    if (in_place && groups - i0 > kThreads * kItems / 4) __syncthreads();
-  }
-  for (int i0 = 0; i0 < n_bias; i0 += kThreads) {
-    const int i = i0 + threadIdx.x, t = i < n_bias ? bid[i] : -1;
-    const uint32_t c = count_of(t);  // 0 for a token that an earlier round has written
-    float z = c ? to_f(logits[t]) : 0.0f;
-    if (in_place) __syncthreads();
-    if (c && allowed(t)) {
-      float s = bval[i];
-      if (twice[(t - base) >> 5] >> ((t - base) & 31) & 1) {  // in the order of the list
-        s = 0.0f;
-        for (int j = 0; j < n_bias; ++j)
-          if (bid[j] == t) s += bval[j];
+#pragma unroll
+    for (int j = 0; j < kBiases; ++j) {
+      const int t = tb[j];
+      if (!cb[j]) continue;
+      if (allowed(t)) {
+        float s = bval[(round * kBiases + j) * kThreads + threadIdx.x];
+        if (twice[(t - base) >> 5] >> ((t - base) & 31) & 1) {  // in the order of the list
+          s = 0.0f;
+          for (int i = 0; i < n_bias; ++i)
+            if (bid[i] == t) s += bval[i];
+        }
+        from_f(penalised(zb[j], cb[j] & ~kBiased) + s, &out[t]);
       }
-      from_f(penalised(z, c & ~kBiased) + s, &out[t]);
+      if (in_place) reinterpret_cast<uint16_t*>(cnt)[t - base] = 0;
     }
-    if (in_place && n_bias - i0 > kThreads) {
-      if (c) reinterpret_cast<uint16_t*>(cnt)[t - base] = 0;
-      __syncthreads();
-    }
+    if (in_place) __syncthreads();
   }
 }
 

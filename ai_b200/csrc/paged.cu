@@ -293,8 +293,7 @@ struct Lay {
   static constexpr int kPart = GT * kW;                 // floats of a state
   static constexpr int kMinRun = 8;                     // units of a CTA's run at least
   static_assert(kTiles * kTile >= kPart * 4, "a warp's last state goes where its tiles were");
-  static_assert(kWarps * kPart >= 2 * GT * kMaxGrid, "the weights of a join go where the first states were");
-  static_assert(2 * kWarps <= 32 && GT <= kWarps, "a lane for every state, a warp for every head");
+  static_assert(2 * kWarps <= 32, "a lane for every state");
 };
 
 // Rows [row, row + box) of head kvh in page id: [HD / 64][box][64] elements in shared memory, 128-byte swizzle.
@@ -393,6 +392,14 @@ AIB_DEV void write_out(E* out, float* lse, float M, float L, float4 a, int d, bo
   if (lse && d == 0) *lse = lse_of(M, L);
 }
 
+// Adds 1 and returns what was there: everything this CTA wrote before its last barrier is visible to who reads after a
+// later ticket.
+AIB_DEV int ticket(int* p) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
+
 struct Owner {  // what a state in shared memory belongs to: heads h0 .. h0 + nh - 1 of b (b < 0: there is none)
   int b, h0, nh, seg0, nblk;
 };
@@ -405,7 +412,6 @@ struct Shared {
   uint64_t full[Lay<HD>::kWarps][kTiles];
   long long wtot[Lay<HD>::kWarps], base;
   Owner own[2 * Lay<HD>::kWarps];  // the warps' first states (parts that began before the piece) and last states
-  float M[GT], L[GT];
   int b, abort, last[2], c0[2], np[2];
 };
 
@@ -820,8 +826,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
 #pragma unroll
     for (int x = 0; x < 2; ++x) cross[x] = (ends[x].seg0 < 0 || ends[x].seg0 + ends[x].nblk > n) && !(x && one);
     if (cross[0] || cross[1]) {
-      __threadfence();
-      __syncthreads();
+      __syncthreads();  // the ticket's release covers the whole CTA's states
       if (threadIdx.x < 2) {
         const Owner w = ends[threadIdx.x];
         bool last = false;
@@ -830,83 +835,61 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
           const int c0 = cta - (w.seg0 < 0 ? (per - 1 - w.seg0) / per : 0), c1 = cta + (w.seg0 + w.nblk - 1) / per;
           sh.c0[threadIdx.x] = c0;
           sh.np[threadIdx.x] = c1 - c0 + 1;
-          last = atomicAdd(&cnt[c0], 1) == c1 - c0;
-          if (last) {
-            cnt[c0] = 0;
-            __threadfence();
-          }
+          last = ticket(&cnt[c0]) == c1 - c0;
+          if (last) cnt[c0] = 0;
         }
         sh.last[threadIdx.x] = last;
       }
       __syncthreads();
-      // A thread has four dimensions of a head and every other state, so that all its loads run at once.
-      float* pm = first;                  // [GT][kMaxGrid]: the states' maxima, then their weights
-      float* pl = pm + GT * kMaxGrid;     // their sums
+      // A thread has four dimensions of a head and every other state, so that up to 16 states are loaded at once.
       for (int x = 0; x < 2; ++x) {
         if (!sh.last[x]) continue;
         const Owner w = ends[x];
-        const int c0 = sh.c0[x], np = sh.np[x], nh = w.nh;
-        auto part_of = [&](int k) {  // the k-th CTA's state
-          return parts_ws + static_cast<long long>(2 * (c0 + k) + (k == 0)) * Y::kPart;
-        };
-        for (int i = threadIdx.x; i < np << head_bits; i += Y::kThreads) {
-          const int h = i & ((1 << head_bits) - 1), k = i >> head_bits;
-          if (h >= nh) continue;
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_of(k) + h * W + HD));
-          pm[h * kMaxGrid + k] = ml.x;
-          pl[h * kMaxGrid + k] = ml.y;
-        }
-        auto weigh = [&]() {  // a warp for every head; all threads come here once
-          __syncthreads();
-          if (warp < nh) {
-            float* m = pm + warp * kMaxGrid;
-            float M = -INFINITY, L = 0.0f;
-            for (int k = lane; k < np; k += 32) M = fmaxf(M, m[k]);
-#pragma unroll
-            for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-            const float z = M == -INFINITY ? 0.0f : M;
-            for (int k = lane; k < np; k += 32) {
-              const float e = exp2f(m[k] - z);
-              m[k] = e;
-              L += e * pl[warp * kMaxGrid + k];
-            }
-            L = warp_sum(L);
-            if (lane == 0) {
-              sh.M[warp] = M;
-              sh.L[warp] = L;
-            }
-          }
-          __syncthreads();
-        };
-        constexpr int kDeep = 8;
-        const int half = lane >> 4;
-        bool weighed = false;
-        for (int i = warp * 16 + (lane & 15); i < nh * (HD / 4); i += Y::kThreads / 2) {  // whole warps go round
+        const int c0 = sh.c0[x], np = sh.np[x], half = lane >> 4;
+        for (int i = warp * 16 + (lane & 15); i < w.nh * (HD / 4); i += Y::kThreads / 2) {  // whole warps go round
+          constexpr int kDeep = 8;
           const int h = i / (HD / 4), d = i % (HD / 4) * 4;
+          float M = -INFINITY, L = 0.0f;
           float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int k0 = half; k0 < np + half; k0 += 2 * kDeep) {
+          for (int k0 = 0; k0 < np; k0 += 2 * kDeep) {
             float4 y[kDeep];
+            float2 ml[kDeep];
+            float m = M;
 #pragma unroll
-            for (int k = 0; k < kDeep; ++k)
-              y[k] = __ldcg(reinterpret_cast<const float4*>(part_of(min(k0 + 2 * k, np - 1)) + h * W + d));
-            if (!weighed) {
-              weigh();
-              weighed = true;
+            for (int k = 0; k < kDeep; ++k) {
+              const int part = min(k0 + 2 * k + half, np - 1);  // the part-th CTA's state
+              const float* p = parts_ws + static_cast<long long>(2 * (c0 + part) + (part == 0)) * Y::kPart + h * W;
+              ml[k] = __ldcg(reinterpret_cast<const float2*>(p + HD));
+              y[k] = __ldcg(reinterpret_cast<const float4*>(p + d));
             }
 #pragma unroll
-            for (int k = 0; k < kDeep; ++k)
-              if (k0 + 2 * k < np) add4(a, pm[h * kMaxGrid + k0 + 2 * k], y[k]);
+            for (int k = 0; k < kDeep; ++k) m = k0 + 2 * k + half < np ? fmaxf(m, ml[k].x) : m;
+            const float z = m == -INFINITY ? 0.0f : m, e = exp2f(M - z);
+            a = make_float4(a.x * e, a.y * e, a.z * e, a.w * e);
+            L *= e;
+            M = m;
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k) {
+              if (k0 + 2 * k + half < np) {
+                const float e = exp2f(ml[k].x - z);
+                add4(a, e, y[k]);
+                L += e * ml[k].y;
+              }
+            }
           }
+          const float mo = __shfl_xor_sync(0xffffffffu, M, 16), m = fmaxf(M, mo);
+          const float e = exp2f(M - (m == -INFINITY ? 0.0f : m));
+          a = make_float4(a.x * e, a.y * e, a.z * e, a.w * e);
+          L *= e;
           a.x += __shfl_xor_sync(0xffffffffu, a.x, 16);
           a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
           a.z += __shfl_xor_sync(0xffffffffu, a.z, 16);
           a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+          L += __shfl_xor_sync(0xffffffffu, L, 16);
           if (half == 0)
             write_out(out + w.b * out_ld + static_cast<long long>(w.h0 + h) * HD,
-                      lse ? lse + static_cast<long long>(w.b) * H + w.h0 + h : nullptr, sh.M[h], sh.L[h], a, d, vec);
+                      lse ? lse + static_cast<long long>(w.b) * H + w.h0 + h : nullptr, m, L, a, d, vec);
         }
-        if (!weighed) weigh();
-        __syncthreads();  // the weights are rewritten next
       }
     }
   }
