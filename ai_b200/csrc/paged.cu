@@ -380,14 +380,16 @@ AIB_DEV void add4(float4& a, float w, float4 x) {
   a.z += w * x.z;
   a.w += w * x.w;
 }
+// No row attended: no maximum and no weights (with NaN scores there is no maximum either, but the sum is NaN).
+AIB_DEV bool nothing(float M, float L) { return M == -INFINITY && L == 0.0f; }
 AIB_DEV float lse_of(float M, float L) {
-  return M == -INFINITY ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+  return nothing(M, L) ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
 }
 // Four neighbouring outputs (from dimension d) of a head from its sums.
 template <typename E>
 AIB_DEV void write_out(E* out, float* lse, float M, float L, float4 a, int d, bool vec) {
-  const float r = M == -INFINITY ? 0.0f : 1.0f / L;
-  store4(out + d, M == -INFINITY ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(a.x * r, a.y * r, a.z * r, a.w * r),
+  const float r = 1.0f / L;
+  store4(out + d, nothing(M, L) ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(a.x * r, a.y * r, a.z * r, a.w * r),
          vec);
   if (lse && d == 0) *lse = lse_of(M, L);
 }
@@ -718,11 +720,12 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int h = 2 * t + hh;
-          const float M = hh ? m1 : m0, L = hh ? l1 : l0, r = M == -INFINITY ? 0.0f : 1.0f / L;
+          const float M = hh ? m1 : m0, L = hh ? l1 : l0, r = 1.0f / L;
+          const bool none = nothing(M, L);
           if (h < nh) {
 #pragma unroll
             for (int d = 0; d < NT; ++d) {
-              const float x = M == -INFINITY ? 0.0f : acc[d][hh] * r, y = M == -INFINITY ? 0.0f : acc[d][2 + hh] * r;
+              const float x = none ? 0.0f : acc[d][hh] * r, y = none ? 0.0f : acc[d][2 + hh] * r;
               from_f32(x, o + h * HD + d * 16);
               from_f32(y, o + h * HD + d * 16 + 8);
             }
@@ -1059,8 +1062,10 @@ int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t tabl
     return fail(AIB_EINVAL, "aib_paged_attn: bad arguments");
   if (B > paged::kMaxBatch) return fail(AIB_ENOTSUP, "aib_paged_attn: at most %d sequences (%d)", paged::kMaxBatch, B);
   const long long room = static_cast<long long>(max_pages) * cache->page;
-  if (room > 0x7fffffffLL || static_cast<long long>(H) * cache->HD > 0x7fffffffLL)
-    return fail(AIB_ENOTSUP, "aib_paged_attn: max_pages * page and H * HD must fit 31 bits");
+  const long long tiles = (H / c.KV + paged::GT - 1) / paged::GT, units = (room + paged::kBlk - 1) / paged::kBlk;
+  if (room > 0x7fffff00LL || static_cast<long long>(H) * cache->HD > 0x7fffffffLL ||
+      units * tiles > (0x7fffffffLL << 6) / B / c.KV)
+    return fail(AIB_ENOTSUP, "aib_paged_attn: max_pages * page and H * HD must fit 31 bits, all the rows of the batch 42");
   const size_t need = paged::attn_ws_bytes(cache->HD);
   if (!ws || ws_bytes < need)
     return fail(AIB_EWORKSPACE, "aib_paged_attn: workspace %zu < %zu bytes", ws_bytes, need);

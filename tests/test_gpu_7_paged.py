@@ -268,6 +268,27 @@ def test_attention_garbage_outside_the_attended_rows(mod):
     assert lib.status() == 0
 
 
+def test_attention_nan_queries_and_keys(mod):
+    """A NaN query head gives NaN there and nowhere else; a NaN key gives NaN to its group."""
+    paged, _, lib = mod
+    for HD, dtype in ((128, "f32"), (64, "bf16")):
+        g = gen(27)
+        pos = [0, 40, 900]
+        c = make_cache(paged, 70, 2, 16, HD, g)
+        table = make_table([p + 1 for p in pos], 16, 70, g)
+        q = torch.randn(3, 8, HD, generator=g, device="cuda").to(DT[dtype])
+        q[:, 1, 3] = float("nan")
+        out, lse = run_attention(paged, c, q, table, pos, 0)
+        assert out[:, 1].isnan().all() and lse[:, 1].isnan().all()
+        keep = [0, 2, 3, 4, 5, 6, 7]
+        assert not out[:, keep].isnan().any()
+        c.k[table[2, 30].long(), 1, 5, 7] = float("nan")
+        out, lse = run_attention(paged, c, q, table, pos, 0)
+        assert out[2, 4:].isnan().all() and lse[2, 4:].isnan().all() and not out[2, [0, 2, 3]].isnan().any()
+        assert not out[:2, keep].isnan().any()
+    assert lib.status() == 0
+
+
 def test_attention_bad_pages_and_positions(mod):
     """Rows on pages outside the pool, or past the table, are left out and recorded."""
     paged, _, lib = mod

@@ -64,7 +64,8 @@ def test_append_refusals(L, bad):
 @pytest.mark.parametrize("bad,code", [(dict(table=None), -1), (dict(pos=None), -1), (dict(q=None), -1),
                                       (dict(out=None), -1), (dict(B=0), -1), (dict(B=4097), -4), (dict(H=3), -1),
                                       (dict(H=0), -1), (dict(window=-1), -1), (dict(dtype=3), -1), (dict(width=0), -1),
-                                      (dict(ws=None), -3), (dict(n=1), -3)])
+                                      (dict(ws=None), -3), (dict(n=1), -3), (dict(width=1 << 27), -4),
+                                      (dict(width=1 << 26, B=4096, ld=1 << 26), -4)])
 def test_attention_refusals(L, bad, code):
     assert attn(L, **bad) == code and L.aib_last_error().startswith(b"aib_paged_attn")
 
