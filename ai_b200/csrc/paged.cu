@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
   constexpr int PQ = sizeof(E) == 4 ? 3 : 1, PP = sizeof(E) == 4 ? 3 : 2;
   constexpr int NT = HD / 16, W = Y::kW, NW = Y::kWarps;
   extern __shared__ uint8_t dyn[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* ring = dyn + (-smem_u32(dyn) & 1023u);
   float* first = reinterpret_cast<float*>(ring + Y::kRing);
   Shared<HD>& sh = *reinterpret_cast<Shared<HD>*>(first + NW * Y::kPart);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
