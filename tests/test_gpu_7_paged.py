@@ -8,7 +8,6 @@ Tolerances count roundings (half a step relative to the value: fp32 2^-24, bf16 
     the sum of p. With bf16 rows the weights are held in two bf16 parts (2^-16) and the output is rounded once.
   adjust: fewer than 8 + (biases of the id) roundings of the terms' magnitudes; bf16 output rounded once.
 """
-import ctypes as C
 
 import numpy as np
 import pytest
