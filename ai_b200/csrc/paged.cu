@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(32 * kAppWarps)
 // error 3.9e-6 with one accumulator, 3.6e-7 so).
 //
 // Measured (B200, captured): 64 sequences of up to 8192 in bf16, 983 MB, 158 us = 6.2 TB/s; one of 131072 in fp32, 537 MB,
-// 95 us = 5.7 TB/s (a few SMs get 12 % less of the memory and finish last); 16 of up to 4096 35 us, of which about 23 us
+// 95 us = 5.7 TB/s (a few SMs get 12 % less of the memory and finish last); 16 of up to 4096 33 us, of which about 21 us
 // are the copies, the rest the sum over the lengths, the first look-up and the joins; one of 517 12.6 us, all latency.
 // Tried and slower: a copying warp for eight computing ones (single units, 190 us for the 64 sequences: it issued too
 // slowly; batches of look-ups, 157 us, but 36 against 25 us for 200 short ones, whose joins held the warps up), 16-byte
