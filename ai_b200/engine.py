@@ -535,11 +535,12 @@ class Engine:
         once for all B tokens. Returns B token lists of max_new tokens each (no early stop at EOS, so the batch
         stays aligned). Uniform draws come from np.random.default_rng(seed), B per step in sequence order.
         page: rows per page (a power of two) of a cache in pages instead of one of `maxt` rows for every sequence; it
-        holds `pages` pages (default: what these prompts and max_new need) and the engine keeps it for later calls.
+        holds `pages` pages (default: what these prompts and max_new need) and the engine keeps it for later calls (one
+        that needs more makes a new one and captures its steps again, which a number of pages given at first avoids).
         Penalties: one number, or one for every prompt, over the most recent 4096 ids of the prompt and its tokens.
         logit_bias: one {id: bias} (or None) for every prompt. mask: int32 [B, ceil(V/32)] (or one row for all), bit j
         of word w = token 32w + j may be drawn; or a function of the tokens so far (a list for every prompt) that gives
-        one before every draw, a grammar's state for instance."""
+        one before every draw, a grammar's state for instance. Every row has to leave a token."""
         B = len(prompts)
         if not 1 <= B <= MAXB:
             raise ValueError(f"generate_batch takes 1..{MAXB} prompts")

@@ -3,7 +3,8 @@
 `pick(logits, temperature, top_p, rng, mask)` keeps the reference signature (rng: numpy Generator; it draws
 exactly one `rng.random()` per sampled row, the same draw `Generator.choice(n, p)` makes, so a seeded rng
 gives the reference's tokens). `sample(...)` adds top-k and repetition/presence/frequency penalties (no
-reference counterpart; see aib_sample in include/ai_b200.h for the order of the steps).
+reference counterpart; see aib_sample in include/ai_b200.h for the order of the steps). `adjust(...)` applies penalties,
+biases and masks to a batch of requests that each have their own, before a draw.
 """
 import numpy as np
 import torch

@@ -490,6 +490,34 @@ def test_graphs_that_share_a_workspace(mod):
     assert lib.status() == 0
 
 
+def test_calls_on_two_streams(mod):
+    """Calls that overlap on the GPU, each with its own workspace, and one without a workspace of its own."""
+    paged, sampler, lib = mod
+    g = gen(25)
+    c = make_cache(paged, 900, 2, 16, 128, g)
+    jobs = []
+    for pos in ([5000, 4], [2000, 2500, 300]):
+        table = make_table([p + 1 for p in pos], 16, 900, g)
+        q = torch.randn(len(pos), 8, 128, generator=g, device="cuda")
+        p = torch.tensor(pos, device="cuda")
+        x = torch.randn(len(pos), 50257, generator=g, device="cuda")
+        prior = torch.randint(0, 500, (len(pos), 300), generator=g, device="cuda", dtype=torch.int32)
+        rep = torch.full((len(pos),), 1.2, device="cuda")
+        jobs.append((torch.cuda.Stream(), paged.workspace(len(pos), 8, c), (q, c, table, p), (x, prior, rep),
+                     paged.attention(q, c, table, p), sampler.adjust(x.clone(), prior=prior, repetition=rep)))
+    torch.cuda.synchronize()
+    got = []
+    for i in range(30):
+        for stream, ws, args, (x, prior, rep), _, _ in jobs:
+            with torch.cuda.stream(stream):
+                got.append((paged.attention(*args, ws=ws if i % 3 else None),
+                            sampler.adjust(x, out=torch.empty_like(x), prior=prior, repetition=rep)))
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(got):
+        assert torch.equal(a, jobs[i % 2][4]) and torch.equal(b, jobs[i % 2][5])
+    assert lib.status() == 0
+
+
 def test_python_refusals(mod):
     """Shapes, types, strides and devices that do not fit raise ValueError before anything is launched."""
     paged, sampler, lib = mod
