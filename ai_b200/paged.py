@@ -98,19 +98,16 @@ def _check_table(what, cache, table, pos):
 
 def _rows(what, t, T, heads, cache, dtype):
     """Returns the address and the token and head strides of rows [T, heads, HD]."""
-    if t.dim() == 3 and t.dtype is dtype and t.get_device() == cache.index:
-        n, h, d = t.shape
-        ts, hs, step = t.stride()
-        if n == T and h == heads and d == cache.HD and step == 1:
-            return t.data_ptr(), ts, hs
-    raise ValueError(f"append: {what} must be {dtype} [{T}, {heads}, {cache.HD}] rows on the cache's device")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != cache.HD or shape[1] != heads or shape[0] != T or stride[2] != 1 or \
+            t.dtype is not dtype or t.get_device() != cache.index:
+        raise ValueError(f"append: {what} must be {dtype} [{T}, {heads}, {cache.HD}] rows on the cache's device")
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _vector(what, t, n, dtypes, cache):
-    if t is None:
-        return None
-    if t.dtype not in dtypes or t.dim() != 1 or t.numel() != n or t.get_device() != cache.index or \
-            not t.is_contiguous():
+def _vector(what, t, n, dtypes, index):
+    """Returns the address of n contiguous elements."""
+    if t.dtype not in dtypes or t.numel() != n or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"append: {what} must be {dtypes[0]} [{n}] on the cache's device")
     return t.data_ptr()
 
@@ -135,17 +132,23 @@ def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=Non
     if (q is None) != (q_out is None):
         raise ValueError("append: q and q_out go together")
     H, qr, qo = 0, _NO_ROWS, _NO_ROWS
-    if q is not None and q.dim() == 3 and q.shape[1]:
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("append: q must be [T, heads, HD] rows like k")
         H = q.shape[1]
+    if H:
         qr, qo = _rows("q", q, T, H, cache, dt), _rows("q_out", q_out, T, H, cache, dt)
     kr, vr = _rows("k", k, T, cache.KV, cache, dt), _rows("v", v, T, cache.KV, cache, dt)
     if cu is None and T != B:
         raise ValueError("append: without cu there must be one token per sequence")
-    cu_at, inv_at = _vector("cu", cu, B + 1, _I32, cache), _vector("inv", inv, HD // 2, _F32, cache)
-    qn_at, kn_at = _vector("qn", qn, HD, _NORM, cache), _vector("kn", kn, HD, _NORM, cache)
+    index = cache.index
+    cu_at = None if cu is None else _vector("cu", cu, B + 1, _I32, index)
+    inv_at = None if inv is None else _vector("inv", inv, HD // 2, _F32, index)
+    qn_at = None if qn is None else _vector("qn", qn, HD, _NORM, index)
+    kn_at = None if kn is None else _vector("kn", kn, HD, _NORM, index)
     if T == 0 or B == 0:
         return q_out
-    with _lib.on_device(cache.index) as stream:
+    with _lib.on_device(index) as stream:
         _lib.call("aib_paged_append", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), cu_at, B, T, H, *qr, *kr,
                   *vr, *qo, _DT[dt], qn_at, kn_at, inv_at, eps, stream)
     return q_out

@@ -536,7 +536,7 @@ def test_python_refusals(mod):
     for bad in (dict(table=z(2, 2, dtype=i32)), dict(table=z(3, 2, dtype=i64)), dict(table=t.cpu()),
                 dict(table=z(3, 4, dtype=i32)[:, ::2]), dict(pos=z(3)), dict(pos=z(6, dtype=i64)[::2]), dict(pos=p.cpu()),
                 dict(k=k.half()), dict(k=k.to(b)), dict(k=z(3, 2, 128)[..., ::2]), dict(v=z(3, 1, 64)),
-                dict(q=z(3, 4, 128)), dict(q_out=None), dict(q_out=z(3, 4, 64).to(b)), dict(q=z(3, 4, 64).cpu()),
+                dict(q=z(3, 4, 128)), dict(q=z(3, 256)), dict(q_out=z(3, 256)), dict(q_out=None), dict(q_out=z(3, 4, 64).to(b)), dict(q=z(3, 4, 64).cpu()),
                 dict(cu=z(3, dtype=i32)), dict(cu=z(4, dtype=i64)), dict(inv=z(64)), dict(inv=z(32).to(b)),
                 dict(qn=z(64)), dict(kn=z(32, dtype=b)), dict(k=z(2, 2, 64), v=z(2, 2, 64), q=None, q_out=None)):
         with pytest.raises(ValueError):
