@@ -58,17 +58,16 @@ def adjust(logits, out=None, prior=None, repetition=None, presence=None, frequen
     ld, step = logits.stride()
     at = out_at = logits.data_ptr()
     if out is None or out is logits:
-        out, out_ld = logits, ld
+        out, out_ld, out_step = logits, ld, step
     else:
         if out.shape != shape or out.dtype != dt or out.device != dev:
             raise ValueError("adjust: out must have the shape, type and device of logits")
         out_ld, out_step = out.stride()
-        step = max(step, out_step)
         out_at, es = out.data_ptr(), logits.element_size()
         if at < out_at + ((B - 1) * out_ld + V) * es and out_at < at + ((B - 1) * ld + V) * es and \
                 (at, ld) != (out_at, out_ld):
             raise ValueError("adjust: out must be logits itself or share no memory with it")
-    if (V > 1 and step != 1) or (B > 1 and out_ld < V):
+    if (V > 1 and (step != 1 or out_step != 1)) or (B > 1 and out_ld < V):
         raise ValueError("adjust: rows must be contiguous and the rows of out apart")
     prior_at, prior_ld, n_prior = _side("prior", prior, B, torch.int32, dev)
     ids_at, ids_ld, nb = _side("bias_ids", bias_ids, B, torch.int32, dev)

@@ -1,0 +1,54 @@
+"""Calls of the paged cache and the logit adjustment that must be refused before anything is launched, and what the
+wrappers hand on, on tensors that only say that they are on a GPU."""
+import numpy as np
+import pytest
+import torch
+
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that reports device cuda:0 (its memory is never touched: nothing is launched)."""
+    is_cuda = property(lambda self: True)
+    device = property(lambda self: torch.device("cuda", 0))
+
+    def get_device(self):
+        return 0
+
+
+def on_gpu(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype).as_subclass(OnGpu)
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """Records the C calls instead of making them."""
+    from ai_b200 import _lib
+    calls = []
+
+    class Device:
+        def __init__(self, index):
+            pass
+
+        def __enter__(self):
+            return 0
+
+        def __exit__(self, *exc):
+            return False
+
+    monkeypatch.setattr(_lib, "on_device", Device)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: calls.append((name, args)))
+    return calls
+
+
+# ---------------------------------------------------------------------------------------------- adjust
+def test_adjust_refuses_rows_of_one_repeated_element(launched):
+    """A row expanded from one element has a column stride of 0, whatever the other tensor's is."""
+    from ai_b200 import sampler
+    one, x = on_gpu(1, 1), on_gpu(1, 70)
+    for kw in (dict(logits=x, out=one.expand(1, 70)), dict(logits=one.expand(1, 70), out=x),
+               dict(logits=on_gpu(3, 1).expand(3, 70), out=on_gpu(3, 70)), dict(logits=one.expand(1, 70))):
+        with pytest.raises(ValueError):
+            sampler.adjust(**kw)
+    assert not launched
+    sampler.adjust(x)
+    sampler.adjust(on_gpu(1, 70).expand(3, 70), out=on_gpu(3, 70))  # one row for all is read, not written
+    assert len(launched) == 2
