@@ -330,6 +330,10 @@ int aib_adjust_logits(const void* logits, int64_t ld, void* out, int64_t out_ld,
   const size_t es = dtype == 0 ? 4 : 2;
   if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % es)
     return fail(AIB_EINVAL, "aib_adjust_logits: logits and out must be aligned to their elements");
+  const Rows2 in{reinterpret_cast<uintptr_t>(logits), static_cast<long long>(V * es), {B, 1}, {ld * static_cast<long long>(es), 0}},
+      to{reinterpret_cast<uintptr_t>(out), static_cast<long long>(V * es), {B, 1}, {out_ld * static_cast<long long>(es), 0}};
+  if (!(out == logits && (B == 1 || ld == out_ld)) && rows_meet(in, to))
+    return fail(AIB_EINVAL, "aib_adjust_logits: out must be logits itself (with the same row stride) or share no memory with it");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == 0 ? adjust::go<float>(logits, ld, out, out_ld, B, V, prior, prior_ld, n_prior, repetition, presence,
                                         frequency, bias_ids, bias_ids_ld, bias, bias_ld, n_bias, mask, mask_ld, s)

@@ -217,6 +217,16 @@ int make_map_3d_u8(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1,
 int make_map(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, int rank, const void* base,
              const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
+// Whether two sets of rows share a byte, and whether the rows of one lie apart (what a kernel writes must). Exact: views
+// that interleave in one buffer are apart although their ranges meet.
+struct Rows2 {
+  uintptr_t base;
+  long long width;         // bytes of a row
+  long long n[2], s[2];    // rows at base + i * s[0] + j * s[1] bytes, i < n[0], j < n[1]
+};
+bool rows_meet(const Rows2& a, const Rows2& b);
+bool rows_apart(const Rows2& a);
+
 // Raise a kernel's dynamic shared-memory limit to the sm_100 per-block maximum (232448 bytes, static +
 // dynamic), once per (kernel, device). A failure is reported and clears the runtime's sticky error.
 bool smem_raised(const void* kernel, int device, bool record);  // true if already recorded

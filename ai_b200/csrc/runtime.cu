@@ -1,4 +1,5 @@
 // Library-wide host runtime: error messages, PDL switch, device status word, tensor-map encoding.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <mutex>
@@ -45,6 +46,71 @@ bool smem_raised(const void* kernel, int device, bool record) {
   std::lock_guard<std::mutex> lock(mu);
   if (record) seen.insert({kernel, device});
   return seen.count({kernel, device}) != 0;
+}
+
+namespace {
+typedef __int128 wide;  // strides are the caller's numbers: no product of them may wrap
+struct Grid2 {
+  wide base, width, n[2], s[2];
+  wide last() const { return base + width + (n[0] - 1) * s[0] + (n[1] - 1) * s[1]; }
+};
+// Strides positive and, where rows lie end to end, the rows joined; dimension 0 has the larger stride. `once`: rows
+// that repeat (stride 0) count once.
+Grid2 canonical(const Rows2& r, bool once) {
+  Grid2 g{static_cast<wide>(r.base), r.width, {r.n[0], r.n[1]}, {r.s[0], r.s[1]}};
+  for (int i = 0; i < 2; ++i) {
+    if (g.s[i] < 0) {
+      g.base += g.s[i] * (g.n[i] - 1);
+      g.s[i] = -g.s[i];
+    }
+    if (g.n[i] == 1 || (once && g.s[i] == 0)) g.n[i] = 1, g.s[i] = 0;
+  }
+  if (g.s[0] < g.s[1]) std::swap(g.n[0], g.n[1]), std::swap(g.s[0], g.s[1]);
+  for (int i = 1; i >= 0; --i)
+    if (g.n[i] > 1 && g.s[i] == g.width) g.width *= g.n[i], g.n[i] = 1, g.s[i] = 0;
+  if (g.s[0] < g.s[1]) std::swap(g.n[0], g.n[1]), std::swap(g.s[0], g.s[1]);
+  return g;
+}
+wide floor_div(wide a, wide b) { return a / b - (a % b < 0); }
+// Rows of one stride s (na from xa, nb from xb): some i, j with xa + i s < xb + j s + wb and xb + j s < xa + i s + wa.
+bool lattices_meet(wide xa, wide na, wide wa, wide xb, wide nb, wide wb, wide s) {
+  const wide d = xb - xa;
+  if (s == 0) return d < wa && -d < wb;
+  const wide lo = std::max(floor_div(-wb - d, s) + 1, 1 - na), hi = std::min(-floor_div(d - wa, s) - 1, nb - 1);
+  return lo <= hi;
+}
+}  // namespace
+
+bool rows_apart(const Rows2& r) {
+  const Grid2 g = canonical(r, false);
+  const wide inner = g.n[1] > 1 ? (g.n[1] - 1) * g.s[1] + g.width : g.width;
+  return (g.n[1] == 1 || g.s[1] >= g.width) && (g.n[0] == 1 || g.s[0] >= inner);
+}
+
+bool rows_meet(const Rows2& ra, const Rows2& rb) {
+  if (ra.n[0] <= 0 || ra.n[1] <= 0 || rb.n[0] <= 0 || rb.n[1] <= 0) return false;
+  Grid2 a = canonical(ra, true), b = canonical(rb, true);
+  if (a.last() <= b.base || b.last() <= a.base) return false;
+  // the dimension with more rows is looked at as a whole, the other row by row
+  auto split = [](const Grid2& g) { return g.n[0] >= g.n[1] ? 0 : 1; };
+  const int la = split(a), lb = split(b);
+  for (wide i = 0; i < a.n[1 - la]; ++i) {
+    const wide xa = a.base + i * a.s[1 - la];
+    for (wide j = 0; j < b.n[1 - lb]; ++j) {
+      const wide xb = b.base + j * b.s[1 - lb];
+      if (xa + a.width + (a.n[la] - 1) * a.s[la] <= xb || xb + b.width + (b.n[lb] - 1) * b.s[lb] <= xa) continue;
+      if (a.s[la] == b.s[lb] || a.n[la] == 1 || b.n[lb] == 1) {
+        if (lattices_meet(xa, a.n[la], a.width, xb, b.n[lb], b.width, std::max(a.s[la], b.s[lb]))) return true;
+      } else if (a.n[la] <= b.n[lb]) {
+        for (wide k = 0; k < a.n[la]; ++k)
+          if (lattices_meet(xa + k * a.s[la], 1, a.width, xb, b.n[lb], b.width, b.s[lb])) return true;
+      } else {
+        for (wide k = 0; k < b.n[lb]; ++k)
+          if (lattices_meet(xa, a.n[la], a.width, xb + k * b.s[lb], 1, b.width, a.s[la])) return true;
+      }
+    }
+  }
+  return false;
 }
 
 int launch_check(const char* what) {

@@ -47,7 +47,7 @@ def adjust(logits, out=None, prior=None, repetition=None, presence=None, frequen
            mask=None):
     """Penalties, biases and grammar masks of a batch of requests, each row with its own parameters (see
     aib_adjust_logits in include/ai_b200.h for the formula): logits [B, V] fp32 or bf16 CUDA rows -> out (default: in
-    place). repetition (> 0) / presence / frequency: fp32 [B] over the ids of prior (int32 [B, P], P <= 32767, -1 =
+    place; else it shares no memory with logits). repetition (> 0) / presence / frequency: fp32 [B] over the ids of prior (int32 [B, P], P <= 32767, -1 =
     empty); bias_ids int32 / bias fp32 [B, n], n <= 1024 (biases of an id listed twice add up, ids outside the
     vocabulary are ignored); mask int32 [B, ceil(V/32)], 1 = allowed. prior, biases and mask may be expanded from one
     row. Returns out."""
@@ -63,10 +63,7 @@ def adjust(logits, out=None, prior=None, repetition=None, presence=None, frequen
         if out.shape != shape or out.dtype != dt or out.device != dev:
             raise ValueError("adjust: out must have the shape, type and device of logits")
         out_ld, out_step = out.stride()
-        out_at, es = out.data_ptr(), logits.element_size()
-        if at < out_at + ((B - 1) * out_ld + V) * es and out_at < at + ((B - 1) * ld + V) * es and \
-                (at, ld) != (out_at, out_ld):
-            raise ValueError("adjust: out must be logits itself or share no memory with it")
+        out_at = out.data_ptr()
     if (V > 1 and (step != 1 or out_step != 1)) or (B > 1 and out_ld < V):
         raise ValueError("adjust: rows must be contiguous and the rows of out apart")
     prior_at, prior_ld, n_prior = _side("prior", prior, B, torch.int32, dev)
