@@ -161,12 +161,13 @@ __global__ void __launch_bounds__(32 * kAppWarps)
   int b, off;
   long long p0;
   if (!find_seq(cu, pos, B, t, &b, &p0, &off) || p0 < 0) return;  // behind the last sequence, or an unused row
-  const long long p = p0 + off;
+  // A position near 2^63 wraps below zero behind its offset: past every table, like the position itself.
+  const long long p = static_cast<long long>(static_cast<unsigned long long>(p0) + static_cast<unsigned>(off));
   // where the token's k and v rows go
   long long row = -1;
   if (v1 > H) {
     const long long pg = p >> c.page_shift;
-    if (pg >= max_pages) {
+    if (p < 0 || pg >= max_pages) {
       if (lane == 0) set_status(AIB_DEV_BAD_POS);
     } else {
       const int id = table[b * table_ld + pg];

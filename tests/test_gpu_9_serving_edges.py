@@ -49,3 +49,22 @@ def test_adjust_rows_that_interleave_in_one_buffer(mod, dtype):
             out.copy_(before[:, V + gap:] if out.data_ptr() != buf.data_ptr() else before[:, :V])
             assert torch.equal(buf, before)
     assert lib.status() == 0
+
+
+# ---------------------------------------------------------------------------------------------- append
+def test_append_positions_at_the_end_of_64_bits(mod):
+    """A first position so far out that its tokens' positions leave 64 bits lies past the table, as all far ones do."""
+    paged, _, lib = mod
+    g = gen(2)
+    k0, v0 = (torch.randn(6, 2, 8, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    for first in (2 ** 63 - 1, 2 ** 63 - 2, 2 ** 62, 2 ** 31, 16):
+        c = paged.Cache(k0.clone(), v0.clone())
+        table = ints([0, 1], [2, 3])
+        k, v = (torch.randn(7, 2, 64, generator=g, device="cuda") for _ in range(2))
+        paged.append(c, table, ints([first, 5], dtype=torch.int64), k, v, cu=ints([0, 4, 7]))
+        assert lib.status() == 104
+        want_k, want_v = k0.clone(), v0.clone()
+        for t in range(3):  # the neighbour's rows are written, and nothing else
+            page, row = 2 + (5 + t) // 8, (5 + t) % 8
+            want_k[page, :, row], want_v[page, :, row] = k[4 + t].bfloat16(), v[4 + t].bfloat16()
+        assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v), first
