@@ -328,8 +328,9 @@ int aib_adjust_logits(const void* logits, int64_t ld, void* out, int64_t out_ld,
     return fail(AIB_ENOTSUP, "aib_adjust_logits: at most %d prior ids and %d biases a row (%d, %d)", adjust::kMaxPrior,
                 adjust::kMaxBias, n_prior, n_bias);
   const size_t es = dtype == 0 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) % es)
-    return fail(AIB_EINVAL, "aib_adjust_logits: logits and out must be aligned to their elements");
+  if (!aligned(es, logits, out) ||
+      !aligned(4, prior, repetition, presence, frequency, bias_ids, bias, mask))
+    return fail(AIB_EINVAL, "aib_adjust_logits: every argument must be aligned to its elements");
   const Rows2 in{reinterpret_cast<uintptr_t>(logits), static_cast<long long>(V * es), {B, 1}, {ld * static_cast<long long>(es), 0}},
       to{reinterpret_cast<uintptr_t>(out), static_cast<long long>(V * es), {B, 1}, {out_ld * static_cast<long long>(es), 0}};
   if (!(out == logits && (B == 1 || ld == out_ld)) && rows_meet(in, to))

@@ -217,6 +217,12 @@ int make_map_3d_u8(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1,
 int make_map(CUtensorMap* map, CUtensorMapDataType dtype, int elem_bytes, int rank, const void* base,
              const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
+// Whether every one of the addresses is a multiple of n (NULL is).
+template <typename... P>
+bool aligned(size_t n, const P*... p) {
+  return (((reinterpret_cast<uintptr_t>(p) % n) == 0) && ...);
+}
+
 // Whether two sets of rows share a byte, and whether the rows of one lie apart (what a kernel writes must). Exact: views
 // that interleave in one buffer are apart although their ranges meet.
 struct Rows2 {

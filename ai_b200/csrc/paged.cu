@@ -1041,9 +1041,8 @@ int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t ta
   if (H < 0 || (H > 0) != (q != nullptr) || (H > 0) != (q_out != nullptr))
     return fail(AIB_EINVAL, "aib_paged_append: q and q_out go with H > 0");
   const size_t es = dtype == 0 ? 4 : 2;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-       reinterpret_cast<uintptr_t>(q_out)) % es)
-    return fail(AIB_EINVAL, "aib_paged_append: rows must be aligned to their elements");
+  if (!aligned(es, q, k, v, q_out) || !aligned(4, table, cu, inv) || !aligned(8, pos) || !aligned(2, qn, kn))
+    return fail(AIB_EINVAL, "aib_paged_append: every argument must be aligned to its elements");
   if (static_cast<long long>(T) * (H + 2LL * c.KV) > 0x7fffffffLL)
     return fail(AIB_ENOTSUP, "aib_paged_append: T * (H + 2 KV) must fit 31 bits");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -1072,6 +1071,9 @@ int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t tabl
   if (!table || !pos || !q || !out || B <= 0 || max_pages <= 0 || table_ld < 0 || window < 0 ||
       (dtype != 0 && dtype != 1) || H <= 0 || H % c.KV || q_ld < 0 || out_ld < 0)
     return fail(AIB_EINVAL, "aib_paged_attn: bad arguments");
+  const size_t es = dtype == 0 ? 4 : 2;
+  if (!aligned(es, q, out) || !aligned(4, table, lse) || !aligned(8, pos))
+    return fail(AIB_EINVAL, "aib_paged_attn: every argument must be aligned to its elements");
   if (B > paged::kMaxBatch) return fail(AIB_ENOTSUP, "aib_paged_attn: at most %d sequences (%d)", paged::kMaxBatch, B);
   const long long room = static_cast<long long>(max_pages) * cache->page;
   const long long tiles = (H / c.KV + paged::GT - 1) / paged::GT, units = (room + paged::kBlk - 1) / paged::kBlk;

@@ -74,3 +74,55 @@ def test_adjust_overlap_is_exact(L, no_gpu):
         seen[bad] += 1
         assert adjust(L, at(x), ld, at(out), out_ld, B, V) == (EINVAL if bad else ECUDA), (x, ld, out, out_ld, B, V)
     assert min(seen) > 500
+
+
+# --------------------------------------------------------------------------------------- paged attention
+def kv(**kw):
+    from ai_b200._lib import PagedKv
+    a = dict(k=1 << 30, v=1 << 31, page_stride=4096, head_stride=2048, row_stride=128, pages=4, page=16, KV=2, HD=128)
+    a.update(kw)
+    return PagedKv(*(a[n] for n, _ in PagedKv._fields_))
+
+
+A = C.c_void_p(1 << 26)
+
+
+def attend(L, c=None, **kw):
+    a = dict(table=A, ld=4, width=4, pos=A, B=2, H=4, q=at(0), q_ld=512, out=at(1024), out_ld=512, dtype=0, lse=None,
+             window=0, ws=None, n=0)
+    a.update(kw)
+    return L.aib_paged_attn(C.byref(c or kv()), a["table"], a["ld"], a["width"], a["pos"], a["B"], a["H"], a["q"],
+                            a["q_ld"], a["out"], a["out_ld"], a["dtype"], a["lse"], a["window"], 0.1, a["ws"], a["n"], None)
+
+
+def append(L, c=None, **kw):
+    a = dict(table=A, ld=4, width=4, pos=A, cu=None, B=2, T=2, H=4, q=at(0), q_s=(512, 128), k=at(10000), k_s=(256, 128),
+             v=at(20000), v_s=(256, 128), q_out=at(30000), qo_s=(512, 128), dtype=0, qn=None, kn=None, inv=None)
+    a.update(kw)
+    return L.aib_paged_append(C.byref(c or kv()), a["table"], a["ld"], a["width"], a["pos"], a["cu"], a["B"], a["T"],
+                              a["H"], a["q"], *a["q_s"], a["k"], *a["k_s"], a["v"], *a["v_s"], a["q_out"], *a["qo_s"],
+                              a["dtype"], a["qn"], a["kn"], a["inv"], 1e-6, None)
+
+
+def off(n):
+    return C.c_void_p((1 << 26) + n)
+
+
+# ------------------------------------------------------------------------------------------- alignment
+@pytest.mark.parametrize("bad", [dict(table=off(2)), dict(pos=off(4)), dict(q=off(2)), dict(out=off(3)), dict(lse=off(2)),
+                                 dict(dtype=1, q=off(1)), dict(dtype=1, out=off(1))])
+def test_attention_refuses_addresses_off_their_elements(L, bad):
+    assert attend(L, **bad) == EINVAL and L.aib_last_error().startswith(b"aib_paged_attn")
+
+
+@pytest.mark.parametrize("bad", [dict(table=off(2)), dict(pos=off(4)), dict(cu=off(1)), dict(inv=off(2)), dict(qn=off(1)),
+                                 dict(kn=off(1)), dict(v=off(2)), dict(dtype=1, q_out=off(1))])
+def test_append_refuses_addresses_off_their_elements(L, bad):
+    assert append(L, **bad) == EINVAL and L.aib_last_error().startswith(b"aib_paged_append")
+
+
+@pytest.mark.parametrize("bad", [dict(prior=off(2), n_prior=3), dict(rep=off(1)), dict(ids=off(2), bias=A, n_bias=3),
+                                 dict(ids=A, bias=off(2), n_bias=3), dict(mask=off(2))])
+def test_adjust_refuses_addresses_off_their_elements(L, bad):
+    assert adjust(L, at(0), 10, at(100), 10, 2, 10, **bad) == EINVAL
+    assert L.aib_last_error().startswith(b"aib_adjust_logits")
