@@ -331,8 +331,9 @@ int aib_adjust_logits(const void* logits, int64_t ld, void* out, int64_t out_ld,
   if (!aligned(es, logits, out) ||
       !aligned(4, prior, repetition, presence, frequency, bias_ids, bias, mask))
     return fail(AIB_EINVAL, "aib_adjust_logits: every argument must be aligned to its elements");
-  const Rows2 in{reinterpret_cast<uintptr_t>(logits), static_cast<long long>(V * es), {B, 1}, {ld * static_cast<long long>(es), 0}},
-      to{reinterpret_cast<uintptr_t>(out), static_cast<long long>(V * es), {B, 1}, {out_ld * static_cast<long long>(es), 0}};
+  const long long row = static_cast<long long>(V * es);
+  const Rows2 in{reinterpret_cast<uintptr_t>(logits), row, {B, 1}, {ld, 0}, es},
+      to{reinterpret_cast<uintptr_t>(out), row, {B, 1}, {out_ld, 0}, es};
   if (!(out == logits && (B == 1 || ld == out_ld)) && rows_meet(in, to))
     return fail(AIB_EINVAL, "aib_adjust_logits: out must be logits itself (with the same row stride) or share no memory with it");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

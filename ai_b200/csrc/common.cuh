@@ -227,8 +227,9 @@ bool aligned(size_t n, const P*... p) {
 // that interleave in one buffer are apart although their ranges meet.
 struct Rows2 {
   uintptr_t base;
-  long long width;         // bytes of a row
-  long long n[2], s[2];    // rows at base + i * s[0] + j * s[1] bytes, i < n[0], j < n[1]
+  long long width;       // bytes of a row
+  long long n[2], s[2];  // rows at base + (i * s[0] + j * s[1]) * unit bytes, i < n[0], j < n[1]
+  size_t unit;
 };
 bool rows_meet(const Rows2& a, const Rows2& b);
 bool rows_apart(const Rows2& a);

@@ -1045,6 +1045,16 @@ int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t ta
     return fail(AIB_EINVAL, "aib_paged_append: every argument must be aligned to its elements");
   if (static_cast<long long>(T) * (H + 2LL * c.KV) > 0x7fffffffLL)
     return fail(AIB_ENOTSUP, "aib_paged_append: T * (H + 2 KV) must fit 31 bits");
+  if (H > 0) {
+    auto rows = [&](const void* p, int heads, int64_t ts, int64_t hs) {
+      return Rows2{reinterpret_cast<uintptr_t>(p), static_cast<long long>(cache->HD * es), {T, heads}, {ts, hs}, es};
+    };
+    const Rows2 to = rows(q_out, H, qo_ts, qo_hs);
+    const bool same = q_out == q && (T == 1 || qo_ts == q_ts) && (H == 1 || qo_hs == q_hs);
+    if (!rows_apart(to) || (!same && rows_meet(to, rows(q, H, q_ts, q_hs))) || rows_meet(to, rows(k, c.KV, k_ts, k_hs)) ||
+        rows_meet(to, rows(v, c.KV, v_ts, v_hs)))
+      return fail(AIB_EINVAL, "aib_paged_append: the rows of q_out must lie apart, and be q's or share no memory with q, k and v");
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto go = [&](auto e) {
     using E = decltype(e);
@@ -1084,6 +1094,12 @@ int aib_paged_attn(const aib_paged_kv* cache, const int32_t* table, int64_t tabl
   if (!ws || ws_bytes < need)
     return fail(AIB_EWORKSPACE, "aib_paged_attn: workspace %zu < %zu bytes", ws_bytes, need);
   if (reinterpret_cast<uintptr_t>(ws) & 15) return fail(AIB_EINVAL, "aib_paged_attn: the workspace must be 16-byte aligned");
+  const long long row = static_cast<long long>(H) * cache->HD * es;
+  const Rows2 from{reinterpret_cast<uintptr_t>(q), row, {B, 1}, {q_ld, 0}, es},
+      to{reinterpret_cast<uintptr_t>(out), row, {B, 1}, {out_ld, 0}, es},
+      sums{reinterpret_cast<uintptr_t>(lse), 4LL * B * H, {lse ? 1 : 0, 1}, {0, 0}, 1};
+  if (!rows_apart(to) || rows_meet(to, from) || rows_meet(sums, from) || rows_meet(sums, to))
+    return fail(AIB_EINVAL, "aib_paged_attn: the rows of out must lie apart, and out, lse and q share no memory");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   auto go = [&](auto fn) {
     return fn(cache, table, table_ld, static_cast<int>(room), pos, B, H, q, q_ld, out, out_ld, lse, window, scale, ws, s);

@@ -57,7 +57,8 @@ struct Grid2 {
 // Strides positive and, where rows lie end to end, the rows joined; dimension 0 has the larger stride. `once`: rows
 // that repeat (stride 0) count once.
 Grid2 canonical(const Rows2& r, bool once) {
-  Grid2 g{static_cast<wide>(r.base), r.width, {r.n[0], r.n[1]}, {r.s[0], r.s[1]}};
+  const wide unit = r.unit;
+  Grid2 g{static_cast<wide>(r.base), r.width, {r.n[0], r.n[1]}, {r.s[0] * unit, r.s[1] * unit}};
   for (int i = 0; i < 2; ++i) {
     if (g.s[i] < 0) {
       g.base += g.s[i] * (g.n[i] - 1);

@@ -123,7 +123,7 @@ def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=Non
     pages. cu (int32 [B+1]): sequence b's tokens are rows cu[b] .. cu[b+1]-1, the first at position pos[b]; rows from
     cu[B] on are left alone. Without cu there is one token per sequence (T == B). qn / kn: q / k norm weights (bf16
     [HD]); inv: fp32 [HD/2] rotation frequencies (None: no rotation, for keys that are rotated already). q [T, H, HD]
-    is normed and rotated into q_out (q_out may be q itself). No two tokens may share a cache row."""
+    is normed and rotated into q_out (q itself, or memory that it shares with none of q, k and v). No two tokens may share a cache row."""
     B, width, ld = _check_table("append", cache, table, pos)
     dt = k.dtype
     if dt not in _DT or k.dim() != 3:
@@ -165,7 +165,7 @@ def workspace(B, H, cache):
 def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws=None):
     """Attention of one new token per sequence (at most 4096): q [B, H, HD] (fp32 or bf16, heads contiguous; normed and
     rotated), its own key and value already in the cache at pos[b]. Attends positions 0 .. pos[b], or with a window the last `window`
-    of them. out: [B, H, HD] like q (allocated when None); lse: optional fp32 [B, H], the log of the summed
+    of them. out: [B, H, HD] like q (allocated when None; not q itself); lse: optional fp32 [B, H], the log of the summed
     exponentials; scale: default HD ** -0.5; ws: from `workspace` (a fresh one per call when None). A row that attends
     nothing gives zeros and lse -inf. Returns out."""
     B, width, ld = _check_table("attention", cache, table, pos)

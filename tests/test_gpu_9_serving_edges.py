@@ -68,3 +68,28 @@ def test_append_positions_at_the_end_of_64_bits(mod):
             page, row = 2 + (5 + t) // 8, (5 + t) % 8
             want_k[page, :, row], want_v[page, :, row] = k[4 + t].bfloat16(), v[4 + t].bfloat16()
         assert torch.equal(c.k, want_k) and torch.equal(c.v, want_v), first
+
+
+def test_outputs_that_share_memory_are_refused(mod):
+    """By the wrappers too, before anything is launched; cuts of one fused row stay allowed."""
+    paged, _, lib = mod
+    g = gen(3)
+    c = paged.Cache(*(torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    table, pos = ints([0, 1], [2, 3]), ints([3, 17], dtype=torch.int64)
+    rows = torch.randn(2, 8, 64, generator=g, device="cuda")
+    q, k, v = rows[:, :4], rows[:, 4:6], rows[:, 6:]
+    square = torch.randn(4, 4, 64, generator=g, device="cuda")
+    before = rows.clone()
+    for bad in (dict(q_out=rows[:, 1:5]), dict(q_out=rows[:, 3:7]), dict(q_out=torch.zeros(1, 4, 64, device="cuda").expand(2, 4, 64)),
+                dict(q=square[:2], q_out=square[:, :2].transpose(0, 1))):
+        with pytest.raises(ValueError):
+            paged.append(c, table, pos, k, v, **{"q": q, **bad})
+    q2 = torch.randn(2, 4, 64, generator=g, device="cuda")
+    for bad in (dict(out=q2), dict(out=torch.empty(2, 4, 64, device="cuda"), lse=q2.view(-1)[:8].view(2, 4))):
+        with pytest.raises(ValueError):
+            paged.attention(q2, c, table, pos, **bad)
+    assert torch.equal(rows, before) and not c.k.any() and not c.v.any()
+    want = paged.append(c, table, pos, k, v, q=q, q_out=torch.empty(2, 4, 64, device="cuda"), qn=torch.ones(64, device="cuda").bfloat16())
+    paged.append(c, table, pos, k, v, q=q, q_out=q, qn=torch.ones(64, device="cuda").bfloat16())
+    assert torch.equal(rows[:, :4], want) and torch.equal(rows[:, 4:], before[:, 4:])
+    assert lib.status() == 0
