@@ -1011,7 +1011,7 @@ static int attend(const aib_paged_kv* c, const int32_t* table, long long table_l
   if (!rc) rc = pool_map(&vmap, c->v, c);
   if (rc) return rc;
   // no more CTAs than the longest sequences the table allows could fill
-  const long long rows = window > 0 ? std::min<long long>(window + kBlk - 1, room) : room;
+  const long long rows = window > 0 ? std::min<long long>(std::min<long long>(window, room) + kBlk - 1, room) : room;
   const long long units = static_cast<long long>(B) * c->KV * tiles * ((rows + kBlk - 1) / kBlk);
   const int grid = static_cast<int>(std::min<long long>(max_grid(), (units + Lay<HD>::kMinRun - 1) / Lay<HD>::kMinRun));
   return launch(attn_kernel<HD, E>, dim3(grid), dim3(Lay<HD>::kThreads), smem_bytes<HD>(), s, "aib_paged_attn", kmap, vmap,

@@ -116,6 +116,7 @@ _NORM = (torch.bfloat16, torch.int16, torch.uint16)
 _F32 = (torch.float32,)
 _I32 = (torch.int32,)
 _NO_ROWS = (None, 0, 0)
+_NO_WINDOW = 2 ** 63 - 1  # of C's type; longer than any cache
 
 
 def append(cache, table, pos, k, v, cu=None, q=None, q_out=None, qn=None, kn=None, inv=None, eps=1e-6):
@@ -199,6 +200,6 @@ def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws
         raise ValueError("attention: ws must come from paged.workspace on the cache's device")
     with _lib.on_device(index) as stream:
         _lib.call("aib_paged_attn", cache.ref, table.data_ptr(), ld, width, pos.data_ptr(), B, H, q.data_ptr(), q_ld,
-                  out.data_ptr(), out_ld, _DT[dt], _addr(lse), window, HD ** -0.5 if scale is None else scale,
+                  out.data_ptr(), out_ld, _DT[dt], _addr(lse), min(window, _NO_WINDOW), HD ** -0.5 if scale is None else scale,
                   ws.data_ptr(), ws.numel(), stream)
     return out

@@ -93,3 +93,24 @@ def test_outputs_that_share_memory_are_refused(mod):
     paged.append(c, table, pos, k, v, q=q, q_out=q, qn=torch.ones(64, device="cuda").bfloat16())
     assert torch.equal(rows[:, :4], want) and torch.equal(rows[:, 4:], before[:, 4:])
     assert lib.status() == 0
+
+
+# ------------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("page,HD", [(16, 64), (1, 128), (2, 128)])
+def test_attention_windows_beyond_the_cache(mod, page, HD):
+    """Windows as large as their type allows are no windows; those up to the length cut where they should."""
+    paged, _, lib = mod
+    g = gen(4)
+    pos, pages = [70, 3, -1, 511], 600 // page + 8
+    c = paged.Cache(*(torch.randn(pages, 2, page, HD, generator=g, device="cuda").bfloat16() for _ in range(2)))
+    table = torch.randperm(pages, generator=g, device="cuda")[:512 // page].to(torch.int32).expand(4, -1).contiguous()
+    q, p = torch.randn(4, 6, HD, generator=g, device="cuda"), torch.tensor(pos, device="cuda")
+    full = paged.attention(q, c, table, p)
+    for window in (512, 513, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 63 - 33, 2 ** 63 - 32, 2 ** 63 - 1, 2 ** 64 + 5):
+        assert torch.equal(paged.attention(q, c, table, p, window=window), full), window
+    ref, lse, mag, dot = opaged.attention(f64(q), f64(c.k), f64(c.v), table.cpu().numpy(), pos, 71, HD ** -0.5)
+    got = f64(paged.attention(q, c, table, p, window=71))
+    # a score: HD + 8 roundings of sum |q||k| and 4 of its own, twice (numerator and sum); 71 + 64 of the sums, twice
+    shift = (HD + 8) * E32 * dot + 4 * E32 * np.abs(np.where(np.isinf(lse), 0, lse))
+    assert (np.abs(got - ref) <= (2 * shift[..., None] + 2 * (71 + 64) * E32) * mag + E32 * np.abs(ref)).all()
+    assert lib.status() == 0

@@ -52,3 +52,19 @@ def test_adjust_refuses_rows_of_one_repeated_element(launched):
     sampler.adjust(x)
     sampler.adjust(on_gpu(1, 70).expand(3, 70), out=on_gpu(3, 70))  # one row for all is read, not written
     assert len(launched) == 2
+
+
+# ------------------------------------------------------------------------------------------- attention
+def fake_cache(paged, KV=2, page=16, HD=64):
+    return paged.Cache(*(on_gpu(4, KV, page, HD, dtype=torch.bfloat16) for _ in range(2)))
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 63 - 32, 2 ** 63 - 1, 2 ** 63, 2 ** 64 + 5, 10 ** 30])
+def test_attention_hands_on_windows_of_any_size(launched, window):
+    """A window beyond 64 bits reaches every row; its lower bits alone would be another window."""
+    from ai_b200 import paged
+    q = on_gpu(1, 4, 64)
+    paged.attention(q, fake_cache(paged), on_gpu(1, 4, dtype=torch.int32), on_gpu(1, dtype=torch.int64), out=on_gpu(1, 4, 64),
+                    window=window, ws=on_gpu(1 << 12, dtype=torch.uint8))
+    (name, args), = launched
+    assert name == "aib_paged_attn" and args[13] == min(window, 2 ** 63 - 1)
