@@ -849,6 +849,7 @@ class PagedBatch(Batch):
 
     def begin(self, adj, rows):
         super().begin(adj, rows)
+        self.ws.zero_()  # a wait that ran out in an earlier batch may have left counters in it
         for b, n in enumerate(rows):
             self.pages.grow(b, n)
 
