@@ -537,6 +537,7 @@ class Engine:
         page: rows per page (a power of two) of a cache in pages instead of one of `maxt` rows for every sequence; it
         holds `pages` pages (default: what these prompts and max_new need) and the engine keeps it for later calls (one
         that needs more makes a new one and captures its steps again, which a number of pages given at first avoids).
+        A failure that the device records in a paged batch raises RuntimeError.
         Penalties: one number, or one for every prompt, over the most recent 4096 ids of the prompt and its tokens.
         logit_bias: one {id: bias} (or None) for every prompt. mask: int32 [B, ceil(V/32)] (or one row for all), bit j
         of word w = token 32w + j may be drawn; or a function of the tokens so far (a list for every prompt) that gives
@@ -573,6 +574,7 @@ class Engine:
                 bt.run(prm)
                 for b, t in enumerate(bt.out_ids.tolist()):
                     out[b].append(t)
+            bt.check()
         finally:
             bt.end()
         return out
@@ -631,6 +633,9 @@ class Batch:
     def begin(self, adj, rows):
         """Before a batch: adj (an Adjustment or None); rows: cache rows that every sequence will fill."""
         self.adj = None if adj is None else adj.load(self)
+
+    def check(self):
+        """After a batch: raises when the device has recorded a failure in it."""
 
     def end(self):
         self.adj = None
@@ -849,9 +854,17 @@ class PagedBatch(Batch):
 
     def begin(self, adj, rows):
         super().begin(adj, rows)
+        with _lib.on_device(self.eng.device.index):
+            self.clean = _lib.status(clear=False) == 0
         self.ws.zero_()  # a wait that ran out in an earlier batch may have left counters in it
         for b, n in enumerate(rows):
             self.pages.grow(b, n)
+
+    def check(self):
+        with _lib.on_device(self.eng.device.index):
+            code = _lib.status(clear=self.clean)  # (one of an earlier call stays, and hides what came after it)
+        if code and self.clean:
+            raise RuntimeError(f"the batch failed on the device: status {code} (AIB_DEV_* in ai_b200.h)")
 
     def end(self):
         super().end()

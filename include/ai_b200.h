@@ -36,7 +36,7 @@ extern "C" {
 #define AIB_ESPACE (-5)     /* output capacity too small (two-pass APIs report need)   */
 
 /* device status codes (aib_status_read) */
-#define AIB_DEV_TIMEOUT_FULL 101  /* GEMV consumer waited too long for a TMA stage          */
+#define AIB_DEV_TIMEOUT_FULL 101  /* GEMV consumer or paged attention waited too long for a copy */
 #define AIB_DEV_TIMEOUT_EMPTY 102 /* GEMV producer waited too long for a free stage         */
 #define AIB_DEV_BAD_TOKEN 103     /* embedding id outside the vocabulary                     */
 #define AIB_DEV_BAD_POS 104       /* KV position outside [0, maxt)                            */

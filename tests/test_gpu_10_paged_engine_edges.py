@@ -31,3 +31,41 @@ def test_counts_left_in_the_workspace_do_not_reach_the_next_batch(eng):
     assert eng.generate_batch(prompts, max_new=20, page=16) == want
     eng._pbt.ws[:1024].view(torch.int32).fill_(1)
     assert eng.generate_batch(prompts, max_new=20, page=16) == want
+
+
+def test_device_failures_of_a_paged_batch_are_raised(eng):
+    """Copies that never come, and a page outside the pool; the next batch is right again."""
+    from ai_b200 import _lib
+    prompts = prompts_of(eng, (40, 9))
+    want = eng.generate_batch(prompts, max_new=6, page=16)
+    _lib.call("aib_debug_knob", 1, 4096)
+    _lib.call("aib_debug_knob", 2, 1)
+    try:
+        with pytest.raises(RuntimeError, match="101"):
+            eng.generate_batch(prompts, max_new=3, page=16)
+    finally:
+        _lib.call("aib_debug_knob", 2, 0)
+        _lib.call("aib_debug_knob", 1, 0)
+    assert _lib.status() == 0  # it has been raised
+    assert eng.generate_batch(prompts, max_new=6, page=16) == want
+
+    def spoil(out):  # between two steps
+        if len(out[0]) == 2:
+            eng._pbt.pages.table[1, 0] = eng._pbt.pages.total
+        return torch.full((1, (eng.V + 31) // 32), -1, dtype=torch.int32)
+
+    with pytest.raises(RuntimeError, match="107"):
+        eng.generate_batch(prompts, max_new=5, page=16, mask=spoil)
+    assert eng.generate_batch(prompts, max_new=6, page=16) == want and _lib.status() == 0
+
+
+def test_a_failure_of_an_earlier_call_is_left_to_its_owner(eng):
+    from ai_b200 import _lib, paged
+    prompts = prompts_of(eng, (40, 9))
+    want = eng.generate_batch(prompts, max_new=6, page=16)
+    c = paged.Cache(*(torch.zeros(2, 1, 8, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    row = torch.zeros(1, 1, 64, device="cuda")
+    paged.append(c, torch.full((1, 1), 9, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"),
+                 row, row)
+    assert eng.generate_batch(prompts, max_new=6, page=16) == want
+    assert _lib.status() == 107
