@@ -231,8 +231,9 @@ __global__ void __launch_bounds__(32 * kAppWarps)
         float a[4], z[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          a[j] = rs * (x[i][j] * ac[j] - x[i][4 + j] * zs[j]);
-          z[j] = rs * (x[i][4 + j] * zc[j] + x[i][j] * as[j]);
+          // without rotation nothing of the partner enters (0 times an infinity would)
+          a[j] = rs * (inv ? x[i][j] * ac[j] - x[i][4 + j] * zs[j] : x[i][j] * ac[j]);
+          z[j] = rs * (inv ? x[i][4 + j] * zc[j] + x[i][j] * as[j] : x[i][4 + j] * zc[j]);
         }
         lo = make_float4(a[0], a[1], a[2], a[3]);
         hi = make_float4(z[0], z[1], z[2], z[3]);

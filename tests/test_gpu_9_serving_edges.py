@@ -114,3 +114,30 @@ def test_attention_windows_beyond_the_cache(mod, page, HD):
     shift = (HD + 8) * E32 * dot + 4 * E32 * np.abs(np.where(np.isinf(lse), 0, lse))
     assert (np.abs(got - ref) <= (2 * shift[..., None] + 2 * (71 + 64) * E32) * mag + E32 * np.abs(ref)).all()
     assert lib.status() == 0
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+def test_append_without_rotation_keeps_neighbours_of_infinities(mod, dtype):
+    """Without rotation no element of a row enters another: rows are copied as they are, whatever they hold. With a
+    norm an infinite element leaves zeros beside itself."""
+    paged, _, lib = mod
+    for HD in (64, 128):
+        g = gen(5)
+        c = paged.Cache(*(torch.zeros(3, 2, 8, HD, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+        k, v, q = (torch.randn(5, n, HD, generator=g, device="cuda").to(DT[dtype]) for n in (2, 2, 3))
+        k[1, 0, 3], k[2, 1, HD // 2 + 5], k[3, 0, 9] = float("inf"), float("-inf"), float("nan")
+        k[4, 1, 0], k[4, 1, HD // 2] = -0.0, 0.0
+        q[0, 2, HD - 1], q[4, 0, 0], v[2, 0, 1] = float("inf"), float("nan"), float("inf")
+        q_out = torch.empty_like(q)
+        paged.append(c, ints([[2, 0]]), ints([6], dtype=torch.int64), k, v, cu=ints([0, 5]), q=q, q_out=q_out)
+        at = [(2, 6), (2, 7), (0, 0), (0, 1), (0, 2)]
+        bits = lambda t: t.view(torch.int16 if t.dtype == torch.bfloat16 else torch.int32)  # noqa: E731
+        for t, (i, r) in enumerate(at):
+            for got, want in ((c.k[i, :, r], k[t].bfloat16()), (c.v[i, :, r], v[t].bfloat16()), (q_out[t], q[t])):
+                nan = want.isnan()
+                assert torch.equal(got.isnan(), nan) and torch.equal(bits(got)[~nan], bits(want)[~nan])
+        w = torch.ones(HD, device="cuda").bfloat16()
+        paged.append(c, ints([[2, 0]]), ints([6], dtype=torch.int64), k, v, cu=ints([0, 5]), kn=w)
+        got = c.k[2, 0, 7]  # token 1, head 0
+        assert got[3].isnan() and not got[:3].any() and not got[4:].any()
+    assert lib.status() == 0
