@@ -7,6 +7,7 @@
 // AIB_DEV_BAD_PAGE, and the row is neither written nor attended.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include "common.cuh"
 
 namespace aib {
@@ -392,7 +393,7 @@ AIB_DEV void add4(float4& a, float w, float4 x) {
   a.z += w * x.z;
   a.w += w * x.w;
 }
-// No row attended: no maximum and no weights (with NaN scores there is no maximum either, but the sum is NaN).
+// No row attended: no maximum and no weights.
 AIB_DEV bool nothing(float M, float L) { return M == -INFINITY && L == 0.0f; }
 AIB_DEV float lse_of(float M, float L) {
   return nothing(M, L) ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
@@ -668,7 +669,10 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
           b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, o));
           b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, o));
         }
-        const float n0 = fmaxf(m0, b0), n1 = fmaxf(m1, b1);
+        // With a row to attend the maximum is finite at least, so that a head whose scores are all -inf (sum 0, NaN by the
+        // definition) can be told from one that attends nothing.
+        const float least = vm ? -FLT_MAX : -INFINITY;
+        const float n0 = fmaxf(fmaxf(m0, b0), least), n1 = fmaxf(fmaxf(m1, b1), least);
         const float z0 = n0 == -INFINITY ? 0.0f : n0, z1 = n1 == -INFINITY ? 0.0f : n1;  // no row so far: weights 0
         const float al0 = exp2f(m0 - z0), al1 = exp2f(m1 - z1);
         m0 = n0;

@@ -141,3 +141,46 @@ def test_append_without_rotation_keeps_neighbours_of_infinities(mod, dtype):
         got = c.k[2, 0, 7]  # token 1, head 0
         assert got[3].isnan() and not got[:3].any() and not got[4:].any()
     assert lib.status() == 0
+
+
+def attend_with_lse(paged, q, c, table, pos, **kw):
+    lse = torch.full(q.shape[:2], 5.0, device="cuda")
+    return paged.attention(q, c, table, ints(pos, dtype=torch.int64), lse=lse, **kw), lse
+
+
+@pytest.mark.parametrize("HD", [64, 128])
+def test_attention_scores_that_are_all_minus_infinity(mod, HD):
+    """No weight is left, so the output is NaN and the log of the sum -inf; rows with a finite score among them count
+    alone; a row that attends nothing keeps zeros."""
+    paged, _, lib = mod
+    g = gen(6)
+    pos, page, pages = [0, 45, 2999, 2999, 700, -1], 16, 480
+    k, v = (torch.randn(pages, 2, page, HD, generator=g, device="cuda").bfloat16() for _ in range(2))
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.zeros(6, 188, dtype=torch.int32, device="cuda")
+    n = [-(-(p + 1) // page) for p in pos]
+    for b in range(5):
+        table[b, :n[b]] = order[sum(n[:b]):sum(n[:b + 1])]
+    q = torch.randn(6, 6, HD, generator=g, device="cuda").bfloat16()
+    q[:, :, 2] = 1.0
+    for b in (0, 1, 2):  # every key of these
+        k[table[b, :n[b]].long(), :, :, 2] = -float("inf")
+    k[table[3, :90].long(), :, :, 2] = -float("inf")  # rows 0 .. 1439 of this one
+    k[table[4, 40].long(), :, 4:9, 2] = -float("inf")
+    c = paged.Cache(k, v)
+    out, lse = attend_with_lse(paged, q, c, table, pos)
+    assert out[:3].isnan().all() and (lse[:3] == -float("inf")).all()
+    assert not out[5].any() and (lse[5] == -float("inf")).all()
+    with np.errstate(invalid="ignore"):
+        ref, rl, mag, _ = opaged.attention(f64(q), f64(k), f64(v), table.cpu().numpy(), [-1, -1, -1, 2999, 700, -1], 0,
+                                           HD ** -0.5)
+    # scores: |q||k| <= sqrt(3 HD) * sqrt(2 HD) and the scale give below 3 sqrt(HD) in size, HD + 8 roundings of it
+    tol = 2 * (HD + 8) * E32 * 3 * HD ** 0.5 + 2 * (3000 + 64) * E32 + 2 * 2.0 ** -16
+    assert (np.abs(f64(out) - ref)[3:5] <= tol * mag[3:5] + EBF * np.abs(ref[3:5])).all()
+    assert np.abs(f64(lse)[3:5] - rl[3:5]).max() <= tol + 4 * E32 * 12
+    # a window that holds no finite score, and one that does
+    out, lse = attend_with_lse(paged, q[3:4], c, table[3:4], [1439], window=300)
+    assert out.isnan().all() and (lse == -float("inf")).all()
+    out, _ = attend_with_lse(paged, q[3:4], c, table[3:4], [1440], window=300)
+    torch.testing.assert_close(out[0].float(), v[table[3, 90].long(), :, 0].repeat_interleave(3, 0).float(), rtol=2 * EBF, atol=0)
+    assert lib.status() == 0
