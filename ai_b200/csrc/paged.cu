@@ -334,6 +334,18 @@ AIB_DEV void split_pair(float lo, float hi, uint32_t* w) {  // lo, hi as N bf16 
     hi -= __uint_as_float(w[k] & 0xFFFF0000u);
   }
 }
+// Two fp32 numbers as three bf16 parts, exactly: 8 bits of the 24 each, cut off and not rounded, so that a number above the
+// largest bf16 one does not round to infinity. An infinity leaves NaN behind. N 1: numbers that are bf16 already.
+template <int N>
+AIB_DEV void split_exact(float lo, float hi, uint32_t* w) {
+  static_assert(N == 1 || N == 3, "24 bits in parts of 8, or 8");
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    w[k] = prmt(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+    lo -= __uint_as_float(__float_as_uint(lo) & 0xFFFF0000u);
+    hi -= __uint_as_float(__float_as_uint(hi) & 0xFFFF0000u);
+  }
+}
 AIB_DEV uint32_t transpose8(uint32_t x) {  // an 8 x 8 matrix of 16-bit elements, a row to four lanes
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -629,8 +641,8 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
       for (int s = 0; s < NT; ++s) {
         const float x[4] = {to_f32(qr[16 * s]), to_f32(qr[16 * s + 1]), to_f32(qr[16 * s + 8]), to_f32(qr[16 * s + 9])};
         uint32_t w0[PQ], w1[PQ];
-        split_pair<PQ>(x[0], x[1], w0);
-        split_pair<PQ>(x[2], x[3], w1);
+        split_exact<PQ>(x[0], x[1], w0);
+        split_exact<PQ>(x[2], x[3], w1);
 #pragma unroll
         for (int k = 0; k < PQ; ++k) bq[s][k][0] = w0[k], bq[s][k][1] = w1[k];
       }

@@ -168,7 +168,8 @@ def attention(q, cache, table, pos, out=None, scale=None, window=0, lse=None, ws
     rotated), its own key and value already in the cache at pos[b]. Attends positions 0 .. pos[b], or with a window the last `window`
     of them. out: [B, H, HD] like q (allocated when None; not q itself); lse: optional fp32 [B, H], the log of the summed
     exponentials; scale: default HD ** -0.5; ws: from `workspace` (a fresh one per call when None). A row that attends
-    nothing gives zeros and lse -inf. Returns out."""
+    nothing gives zeros and lse -inf; a head whose scores are all -inf gives NaN and lse -inf. Infinite queries, and
+    infinite keys or values in attended rows, may give NaN where they meet. Returns out."""
     B, width, ld = _check_table("attention", cache, table, pos)
     HD, index, dt = cache.HD, cache.index, q.dtype
     if q.dim() != 3 or dt not in _DT or q.get_device() != index:

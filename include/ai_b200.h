@@ -259,8 +259,11 @@ int aib_paged_append(const aib_paged_kv* cache, const int32_t* table, int64_t ta
                      const float* inv, float eps, void* stream);
 /* Attention of one new token per sequence, its own k and v already in the cache: q [B, H, HD] (normed and rotated;
  * rows at q_ld) attends positions max(0, pos[b] - window + 1) .. pos[b] (window 0: 0 .. pos[b]); out [B, H, HD] (rows
- * at out_ld), lse fp32 [B, H] or NULL = log of the sum of exp(scale * q.k). A row that attends nothing gives zeros and
- * lse -inf; a head whose scores are all -inf gives NaN and lse -inf. out, lse and q share no memory. dtype of q and out: 0 fp32 (products and sums as accurate as fp32), 1 bf16. H a multiple of KV.
+ * at out_ld), lse fp32 [B, H] or NULL = log of the sum of exp(scale * q.k). dtype of q and out: 0 fp32 (products and
+ * sums as accurate as fp32), 1 bf16. H a multiple of KV. out, lse and q share no memory.
+ * A row that attends nothing gives zeros and lse -inf; a head whose scores are all -inf gives NaN and lse -inf.
+ * Infinities among attended rows: an infinite q gives its head NaN, with fp32 rows so may an infinite key (a score of
+ * -inf, too), and an infinite value gives its dimension an infinity or NaN.
  * ws: aib_paged_attn_workspace(...) bytes, 16-byte aligned, zero-filled once (left zeroed where it must be, unless a
  * wait ran out: AIB_DEV_TIMEOUT_FULL); calls that may overlap on the GPU need separate ones. B <= 4096. */
 size_t aib_paged_attn_workspace(int B, int H, int KV, int HD);

@@ -184,3 +184,32 @@ def test_attention_scores_that_are_all_minus_infinity(mod, HD):
     out, _ = attend_with_lse(paged, q[3:4], c, table[3:4], [1440], window=300)
     torch.testing.assert_close(out[0].float(), v[table[3, 90].long(), :, 0].repeat_interleave(3, 0).float(), rtol=2 * EBF, atol=0)
     assert lib.status() == 0
+
+
+@pytest.mark.parametrize("HD", [64, 128])
+def test_attention_fp32_queries_at_the_end_of_their_range(mod, HD):
+    """fp32 queries above the largest bf16 number (3.39e38): the scores are those of the definition. Infinite ones make
+    their heads NaN and no others."""
+    paged, _, lib = mod
+    g = gen(7)
+    pos, page = [40, 700, 5], 16
+    k = torch.randn(64, 2, page, HD, generator=g, device="cuda")
+    k[..., 1] *= 1e-38 / HD ** 0.5  # what meets the large element
+    k[..., 4] = k[..., 4].abs() + 0.25
+    c = paged.Cache(k.bfloat16(), torch.randn(64, 2, page, HD, generator=g, device="cuda").bfloat16())
+    table = torch.randperm(64, generator=g, device="cuda")[:44].to(torch.int32).expand(3, -1).contiguous()
+    top = torch.finfo(torch.float32).max
+    q = torch.randn(3, 4, HD, generator=g, device="cuda")
+    q[0, :, 1] = torch.tensor([top, -top, 3.3953e38, 3.3895e38], device="cuda")
+    q[1, :, 1] = torch.tensor([3.4e38, -3.392e38, 3.2e38, -top], device="cuda")
+    out, lse = attend_with_lse(paged, q, c, table, pos)
+    ref, rl, mag, dot = opaged.attention(f64(q), f64(c.k), f64(c.v), table.cpu().numpy(), pos, 0, HD ** -0.5)
+    shift = (HD + 8) * E32 * dot + 4 * E32 * np.abs(rl)
+    assert (np.abs(f64(out) - ref) <= (2 * shift[..., None] + 2 * (701 + 64) * E32) * mag + E32 * np.abs(ref)).all()
+    assert (np.abs(f64(lse) - rl) <= shift + (701 + 64) * E32 + 4 * E32 * (1 + np.abs(rl))).all()
+    q[:, 1, 4] = -float("inf")
+    q[:, 2, 4] = float("inf")
+    out, lse = attend_with_lse(paged, q, c, table, pos)
+    assert out[:, 1:3].isnan().all() and not torch.isfinite(lse[:, 1:3]).any()
+    assert torch.isfinite(out[:, [0, 3]]).all() and torch.isfinite(lse[:, [0, 3]]).all()
+    assert lib.status() == 0
