@@ -873,7 +873,14 @@ class PagedBatch(Batch):
 
     def _prompt(self, b, tokens):
         eng, n = self.eng, len(tokens)
-        eng.ctx = []  # the engine's own cache is the workplace
+        own = eng.kv[:, :, :, :min(n, len(eng.ctx))].clone()  # the engine's own cache is the workplace
+        try:
+            self._fill(b, tokens)
+        finally:
+            eng.kv[:, :, :, :own.shape[3]].copy_(own)
+
+    def _fill(self, b, tokens):
+        eng, n = self.eng, len(tokens)
         eng._prompt(tokens, 0)
         at = torch.zeros(1, dtype=torch.int64, device=eng.device)
         cu = torch.tensor([0, n], dtype=torch.int32, device=eng.device)

@@ -69,3 +69,25 @@ def test_a_failure_of_an_earlier_call_is_left_to_its_owner(eng):
                  row, row)
     assert eng.generate_batch(prompts, max_new=6, page=16) == want
     assert _lib.status() == 107
+
+
+def test_the_engines_own_sequence_survives_a_paged_batch(eng):
+    """Prompts of a paged batch run in the engine's cache; what was in it is put back, also when the batch fails."""
+    text, tail = prompts_of(eng, (40, 7), seed=5)
+    first = eng.process(text, 0)
+    kept = eng.kv[:, :, :, :40].clone()
+    want = eng.process(tail, 40)
+    assert torch.equal(eng.kv[:, :, :, :40], kept)
+    for lens in ((60, 3), (5, 9)):  # longer and shorter than the sequence
+        assert eng.process(text, 0) == first
+        prompts = prompts_of(eng, lens)
+        alone = eng.generate_batch(prompts, max_new=4)
+        assert eng.generate_batch(prompts, max_new=4, page=8) == alone
+        assert eng.ctx == text and torch.equal(eng.kv[:, :, :, :40], kept)
+        with pytest.raises(ValueError):
+            eng.generate_batch(prompts, max_new=4, page=8, mask=lambda out: torch.zeros(1, 1))
+        with pytest.raises(ZeroDivisionError):
+            eng.generate_batch(prompts, max_new=4, page=8,
+                               mask=lambda out: 1 // 0 if len(out[0]) else torch.full((1, (eng.V + 31) // 32), -1,
+                                                                                      dtype=torch.int32))
+        assert eng.process(tail, 40) == want
