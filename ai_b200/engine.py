@@ -588,7 +588,7 @@ class Engine:
             raise ValueError(f"{need} pages of {page} rows are needed, the pool has {pages}")
         bt = getattr(self, "_pbt", None)
         if bt is None or bt.B != B or bt.page != page or bt.pages.total < need or pages not in (None, bt.pages.total):
-            self._pbt = None  # the old pool is freed before the new one is made
+            bt = self._pbt = None  # the old pool is freed before the new one is made
             self._pbt = bt = PagedBatch(self, B, page, pages or need)
         return bt
 

@@ -68,3 +68,26 @@ def test_attention_hands_on_windows_of_any_size(launched, window):
                     window=window, ws=on_gpu(1 << 12, dtype=torch.uint8))
     (name, args), = launched
     assert name == "aib_paged_attn" and args[13] == min(window, 2 ** 63 - 1)
+
+
+# --------------------------------------------------------------------------------------- engine's pools
+def test_a_pool_is_freed_before_the_next_one_is_made(monkeypatch):
+    """A pool may take most of the memory: there are never two."""
+    import weakref
+    from ai_b200 import engine
+    alive = weakref.WeakSet()
+
+    class Pool:
+        def __init__(self, eng, B, page, pages):
+            assert not alive, "the old pool is still there"
+            alive.add(self)
+            self.B, self.page, self.pages = B, page, type("Pages", (), {"total": pages})()
+
+    monkeypatch.setattr(engine, "PagedBatch", Pool)
+    eng = engine.Engine.__new__(engine.Engine)
+    for B, page, pages, rows in ((2, 16, None, [17, 5]), (2, 16, None, [40, 5]), (3, 16, 9, [16, 16, 16]), (3, 8, None, [8] * 3)):
+        bt = eng._paged_batch(B, page, pages, rows)
+        assert bt.B == B and bt.page == page
+        del bt
+    same = eng._paged_batch(3, 8, None, [8, 8, 1])
+    assert eng._paged_batch(3, 8, None, [1, 1, 1]) is same
