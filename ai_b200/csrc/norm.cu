@@ -77,14 +77,15 @@ __global__ void advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* o
 }
 
 // Batched decode: sequence b's sampled id becomes its next input and its position advances by one; its ring of prior ids
-// (if any) takes the id in.
-__global__ void batch_advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, int32_t* prior,
-                                     long long prior_ld, int n_prior) {
+// (if any) takes the id in. keep_unused: rows at a negative position, unused ones of a paged batch, are left alone.
+__global__ void batch_advance_kernel(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, bool keep_unused,
+                                     int32_t* prior, long long prior_ld, int n_prior) {
   pdl_wait();
   for (int b = threadIdx.x; b < B; b += blockDim.x) {
     const int64_t tok = out_ids[b], p = pos[b] + 1;
+    if (keep_unused && p <= 0) continue;
     next_ids[b] = tok;
-    if (prior && n_prior > 0 && p >= 0) prior[b * prior_ld + p % n_prior] = static_cast<int32_t>(tok);
+    if (prior && n_prior > 0) prior[b * prior_ld + p % n_prior] = static_cast<int32_t>(tok);
     pos[b] = p;
   }
   pdl_trigger();
@@ -117,14 +118,17 @@ int aib_step_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, in
 }
 
 int aib_batch_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, void* stream) {
-  return aib_batch_advance_prior(pos, next_ids, out_ids, B, nullptr, 0, 0, stream);
+  if (!pos || !next_ids || !out_ids || B <= 0) return fail(AIB_EINVAL, "aib_batch_advance: bad arguments");
+  return launch(norm::batch_advance_kernel, dim3(1), dim3(32), 0, static_cast<cudaStream_t>(stream),
+                "aib_batch_advance", pos, next_ids, out_ids, B, false, static_cast<int32_t*>(nullptr), 0LL, 0);
 }
 
 int aib_batch_advance_prior(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, int32_t* prior,
                             int64_t prior_ld, int n_prior, void* stream) {
   if (!pos || !next_ids || !out_ids || B <= 0 || n_prior < 0 || prior_ld < 0)
-    return fail(AIB_EINVAL, "aib_batch_advance: bad arguments");
+    return fail(AIB_EINVAL, "aib_batch_advance_prior: bad arguments");
   return launch(norm::batch_advance_kernel, dim3(1), dim3(32), 0, static_cast<cudaStream_t>(stream),
-                "aib_batch_advance", pos, next_ids, out_ids, B, prior, static_cast<long long>(prior_ld), n_prior);
+                "aib_batch_advance_prior", pos, next_ids, out_ids, B, true, prior, static_cast<long long>(prior_ld), n_prior);
 }
+
 }  // extern "C"

@@ -183,7 +183,7 @@ int aib_step_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, in
 /* Batched decode bookkeeping: next_ids[b] = out_ids[b]; pos[b] += 1 for b < B. */
 int aib_batch_advance(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, void* stream);
 /* The same, and prior[b * prior_ld + new pos[b] % n_prior] = the id (a ring of recent ids for every sequence, as
- * aib_step_advance's; prior NULL: none). */
+ * aib_step_advance's; prior NULL: none); rows at a negative position, unused ones of a paged batch, are left alone. */
 int aib_batch_advance_prior(int64_t* pos, int64_t* next_ids, const int64_t* out_ids, int B, int32_t* prior,
                             int64_t prior_ld, int n_prior, void* stream);
 

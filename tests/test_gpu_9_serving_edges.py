@@ -213,3 +213,64 @@ def test_attention_fp32_queries_at_the_end_of_their_range(mod, HD):
     assert out[:, 1:3].isnan().all() and not torch.isfinite(lse[:, 1:3]).any()
     assert torch.isfinite(out[:, [0, 3]]).all() and torch.isfinite(lse[:, [0, 3]]).all()
     assert lib.status() == 0
+
+
+# ------------------------------------------------------------------------------------------- the step
+def test_unused_rows_stay_unused_as_the_batch_advances(mod):
+    """A negative position marks an unused row: a step leaves its position, its id and its ring alone."""
+    _, _, lib = mod
+    from ai_b200._lib import ptr, stream_ptr
+    for B in (3, 16, 70):
+        pos = torch.arange(B, device="cuda") * 3
+        pos[1::3] = -1
+        pos[2::5] = -2 ** 62
+        ids, out_ids = torch.arange(B, device="cuda") + 100, torch.arange(B, device="cuda") + 500
+        ring = torch.full((B, 8), -1, dtype=torch.int32, device="cuda")
+        used = pos >= 0
+        want_pos, want_ids, want_ring = torch.where(used, pos + 2, pos), torch.where(used, out_ids, ids), ring.clone()
+        for b in torch.nonzero(used).flatten().tolist():
+            for s in (1, 2):
+                want_ring[b, (pos[b].item() + s) % 8] = 500 + b
+        for r in (ring, None):
+            p, i = pos.clone(), ids.clone()
+            for _ in range(2):
+                lib.call("aib_batch_advance_prior", ptr(p), ptr(i), ptr(out_ids), B, ptr(r), 8 if r is not None else 0,
+                         8 if r is not None else 0, stream_ptr())
+            assert torch.equal(p, want_pos) and torch.equal(i, want_ids)
+        assert torch.equal(ring, want_ring)
+        p, i = pos.clone(), ids.clone()
+        lib.call("aib_batch_advance", ptr(p), ptr(i), ptr(out_ids), B, stream_ptr())  # this one knows no unused rows
+        assert torch.equal(p, pos + 1) and torch.equal(i, out_ids)
+    assert lib.status() == 0
+
+
+def test_a_captured_step_with_unused_rows(mod):
+    """Append, attention and advance replayed: the unused row writes to no page, its table's entries notwithstanding."""
+    paged, _, lib = mod
+    from ai_b200._lib import ptr, stream_ptr
+    g = gen(8)
+    c = paged.Cache(*(torch.zeros(6, 1, 8, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    table = ints([0, 1], [2, 3], [4, 5])
+    pos, ids, out_ids = ints([3, -1, 6], dtype=torch.int64), ints([0, 0, 0], dtype=torch.int64), ints([7, 8, 9], dtype=torch.int64)
+    ring, ws = torch.full((3, 4), -1, dtype=torch.int32, device="cuda"), paged.workspace(3, 2, c)
+    q, k, v = (torch.randn(3, n, 64, generator=g, device="cuda") for n in (2, 1, 1))
+    out = torch.full((3, 2, 64), 5.0, device="cuda")
+
+    def step():
+        paged.append(c, table, pos, k, v)
+        paged.attention(q, c, table, pos, out=out, ws=ws)
+        lib.call("aib_batch_advance_prior", ptr(pos), ptr(ids), ptr(out_ids), 3, ptr(ring), 4, 4, stream_ptr())
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(4):
+        graph.replay()
+    assert pos.tolist() == [8, -1, 11] and ids.tolist() == [7, 0, 9] and ring[1].tolist() == [-1] * 4
+    assert not c.k[2:4].any() and not c.v[2:4].any() and not out[1].any()
+    want = k.bfloat16()
+    for b, first in ((0, 3), (2, 6)):
+        for p in range(first, first + 5):
+            assert torch.equal(c.k[table[b, p // 8].item(), :, p % 8], want[b])
+    assert lib.status() == 0
