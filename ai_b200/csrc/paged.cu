@@ -946,8 +946,19 @@ static int check_kv(const char* what, const aib_paged_kv* c, Kv* o) {
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) ||
       ((c->page_stride | c->head_stride | c->row_stride) & 7))
     return fail(AIB_EINVAL, "%s: cache rows must start on 16-byte boundaries", what);
-  if ((c->pages > 1 && c->page_stride < c->HD) || (c->KV > 1 && c->head_stride < c->HD) ||
-      (c->page > 1 && c->row_stride < c->HD))
+  // from the smallest stride on, every one steps over all that lies within it
+  long long n[3] = {c->pages, c->KV, c->page}, st[3] = {c->page_stride, c->head_stride, c->row_stride};
+  if (st[0] < st[1]) std::swap(st[0], st[1]), std::swap(n[0], n[1]);
+  if (st[1] < st[2]) std::swap(st[1], st[2]), std::swap(n[1], n[2]);
+  if (st[0] < st[1]) std::swap(st[0], st[1]), std::swap(n[0], n[1]);
+  __int128 within = c->HD;
+  bool apart = true;
+  for (int i = 2; i >= 0; --i) {
+    if (n[i] == 1) continue;
+    apart = apart && st[i] >= within;
+    within += static_cast<__int128>(n[i] - 1) * st[i];
+  }
+  if (!apart)
     return fail(AIB_EINVAL, "%s: cache rows overlap", what);
   *o = Kv{c->k, c->v, c->page_stride, c->head_stride, c->row_stride, c->pages, c->KV, __builtin_ctz(c->page)};
   return AIB_OK;

@@ -37,8 +37,11 @@ class Cache:
             raise ValueError("cache: HD must be 64 or 128 and the rows of a page a power of two")
         if k.stride(3) != 1 or any(s % 8 for s in k.stride()[:3]) or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("cache: rows must be contiguous and 16-byte aligned")
-        if any(n > 1 and s < self.HD for n, s in zip(k.shape[:3], k.stride()[:3])):
-            raise ValueError("cache: rows must not overlap")
+        within = self.HD  # from the smallest stride on, every one steps over all that lies within it
+        for s, n in sorted(zip(k.stride()[:3], k.shape[:3])):
+            if n > 1 and s < within:
+                raise ValueError("cache: rows must not overlap")
+            within += (n - 1) * s
         self.k, self.v, self.device, self.index = k, v, k.device, k.get_device()
         self.desc = PagedKv(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), self.pages, self.page,
                             self.KV, self.HD)

@@ -195,3 +195,27 @@ def test_attention_takes_rows_that_interleave_apart(L, no_gpu):
     for ok in (dict(), dict(out=at(512), out_ld=1024, q_ld=1024), dict(q=at(512), q_ld=1030, out=at(0), out_ld=1030),
                dict(lse=at(2048)), dict(q_ld=0, out=at(512)), dict(lse=at(512), q_ld=1024, out=at(4096))):
         assert attend(L, **ok) == ECUDA, ok
+
+
+# ------------------------------------------------------------------------------------------------ pools
+OVERLAPS = [dict(page_stride=2048, head_stride=2048),                      # a page's second head is the next page's first
+            dict(page_stride=128, head_stride=2048, row_stride=128),
+            dict(page_stride=4096, head_stride=128, row_stride=128),        # heads among the rows
+            dict(page_stride=4096, head_stride=2048 - 128, row_stride=128), # the last row is the next head's first
+            dict(page_stride=4096 - 8, head_stride=2048, row_stride=128),
+            dict(page_stride=2048, head_stride=128, row_stride=256, pages=2, page=16)]
+APART = [dict(), dict(head_stride=128, row_stride=256), dict(page_stride=8192, head_stride=128, row_stride=512),
+         dict(page_stride=128, head_stride=512 * 16, row_stride=512), dict(KV=1, head_stride=8, page_stride=2048),
+         dict(pages=1, page_stride=0), dict(page=1, row_stride=0, head_stride=128, page_stride=256),
+         dict(page_stride=2 ** 61, head_stride=2048)]
+
+
+@pytest.mark.parametrize("bad", OVERLAPS)
+def test_pools_whose_rows_overlap_are_refused(L, bad):
+    assert append(L, kv(**bad)) == EINVAL and attend(L, kv(**bad)) == EINVAL
+    assert b"overlap" in L.aib_last_error()
+
+
+def test_pools_of_every_order_are_taken(L, no_gpu):
+    for ok in APART:
+        assert append(L, kv(**ok)) == ECUDA, ok

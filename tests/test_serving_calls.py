@@ -91,3 +91,16 @@ def test_a_pool_is_freed_before_the_next_one_is_made(monkeypatch):
         del bt
     same = eng._paged_batch(3, 8, None, [8, 8, 1])
     assert eng._paged_batch(3, 8, None, [1, 1, 1]) is same
+
+
+def test_a_cache_of_rows_that_overlap_is_refused():
+    from ai_b200 import paged
+    pool = on_gpu(1 << 16, dtype=torch.bfloat16)
+    for size, stride in (((4, 2, 16, 64), (1024, 1024, 64, 1)), ((4, 2, 16, 64), (2048, 64, 64, 1)),
+                         ((4, 2, 16, 64), (64, 1024, 64, 1)), ((2, 2, 16, 128), (4096 - 8, 2048, 128, 1))):
+        with pytest.raises(ValueError):
+            paged.Cache(*(pool.as_strided(size, stride),) * 2)
+    for size, stride in (((4, 2, 16, 64), (2048, 1024, 64, 1)), ((4, 2, 16, 64), (2048, 64, 128, 1)),
+                         ((4, 2, 16, 64), (64, 4096, 256, 1)), ((1, 2, 16, 64), (0, 1024, 64, 1)),
+                         ((4, 1, 1, 64), (64, 0, 0, 1))):
+        paged.Cache(*(pool.as_strided(size, stride),) * 2)
