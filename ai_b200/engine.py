@@ -551,18 +551,19 @@ class Engine:
             self._validate_process(list(p), 0)
             if len(p) + max_new > self.maxt:
                 raise ValueError(f"prompt + max_new longer than the context {self.maxt}")
+        rows = [len(p) + max(1, max_new) - 1 for p in prompts]  # the last token drawn is not cached
         adj = Adjustment.of(self, prompts, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, mask)
         if page is None:
             if pages is not None:
                 raise ValueError("pages go with a page size")
             bt = self._batch(B)
         else:
-            bt = self._paged_batch(B, page, pages, [len(p) + max(1, max_new) for p in prompts])
+            bt = self._paged_batch(B, page, pages, rows)
         prm = sampler.params(temperature, top_k, top_p)
         rng = np.random.default_rng(seed)
         out = [[] for _ in range(B)]
         try:
-            bt.begin(adj, [len(p) + max(1, max_new) for p in prompts])
+            bt.begin(adj, rows)
             bt.constrain(out)
             for b, p in enumerate(prompts):
                 us = [rng.random()] if temperature > 0 else None

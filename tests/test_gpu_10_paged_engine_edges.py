@@ -91,3 +91,14 @@ def test_the_engines_own_sequence_survives_a_paged_batch(eng):
                                mask=lambda out: 1 // 0 if len(out[0]) else torch.full((1, (eng.V + 31) // 32), -1,
                                                                                       dtype=torch.int32))
         assert eng.process(tail, 40) == want
+
+
+def test_pages_hold_the_rows_that_are_written_and_no_more(eng):
+    """The last token drawn gets no row: a prompt that fills its pages, or the context, leaves room for one draw."""
+    for lens, max_new, page, pages in (((16, 32), 1, 16, 3), ((13, 5), 4, 8, 3), ((128,), 0, 16, 8), ((127, 9), 1, 32, 5)):
+        prompts = prompts_of(eng, lens)
+        want = eng.generate_batch(prompts, max_new=max_new)
+        assert eng.generate_batch(prompts, max_new=max_new, page=page, pages=pages) == want
+        if pages > len(lens):
+            with pytest.raises(ValueError):
+                eng.generate_batch(prompts, max_new=max_new, page=page, pages=pages - 1)
