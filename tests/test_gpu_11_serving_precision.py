@@ -3,9 +3,9 @@
 Attention: products and sums as accurate as fp32. In the root mean square over the outputs, relative to theirs, that is
   (8 + 4 rms|s|) 2^-24, s the scores in nats:
 a weight carries about 8 roundings of its own (exponential, two scalings, its parts, the sums over rows and states) and its
-score about 4 of the score's size. Weights held in two bf16 parts are off by about 2^-9 / sqrt(3) twice over, 0.9e-6, which
-is above it where the scores are small; queries in two parts shift a score by 0.9e-6 of its size, above it where they are
-large; a single accumulator over all rows gave 3.9e-6 at 131072 rows.
+score about 4 of the score's size. Weights held in two bf16 parts instead of three give 2.0e-6 to 2.6e-6 at scores of 0.1 and
+1, above it; queries in two parts 2.5e-6 at scores of 1 and 2.9e-6 to 8.5e-6 at 5, above it; a single accumulator over all
+rows gave 3.9e-6 at 131072 rows.
 """
 import numpy as np
 import pytest

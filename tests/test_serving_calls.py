@@ -104,3 +104,22 @@ def test_a_cache_of_rows_that_overlap_is_refused():
                          ((4, 2, 16, 64), (64, 4096, 256, 1)), ((1, 2, 16, 64), (0, 1024, 64, 1)),
                          ((4, 1, 1, 64), (64, 0, 0, 1))):
         paged.Cache(*(pool.as_strided(size, stride),) * 2)
+
+
+# --------------------------------------------------------------------------------------- current device
+@pytest.mark.parametrize("current,tensors", [(0, 0), (0, 3), (5, 2)])
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch, current, tensors):
+    """The device of the tensors is made current for a call, with its own stream, and the old one again afterwards, also
+    when the call is refused."""
+    from ai_b200 import _lib
+    state = [current]
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: state[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 1000 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: state.__setitem__(0, i))
+    with _lib.on_device(tensors) as stream:
+        assert state[0] == tensors and stream == 1000 + tensors
+    assert state[0] == current
+    with pytest.raises(ValueError):
+        with _lib.on_device(tensors):
+            raise ValueError
+    assert state[0] == current
