@@ -13,6 +13,7 @@ from . import build as _build
 LIB_PATH = _build.LIB
 
 AIB_OK, AIB_EINVAL, AIB_ECUDA, AIB_EWORKSPACE, AIB_ENOTSUP, AIB_ESPACE = 0, -1, -2, -3, -4, -5
+DEV_SAMPLER_CAP = 105  # AIB_DEV_SAMPLER_CAP
 
 P = C.c_void_p
 I32, I64, F32, SZ = C.c_int32, C.c_int64, C.c_float, C.c_size_t

@@ -22,9 +22,11 @@ namespace aib {
 
 // ------------------------------------------------------------------------------------------ status
 // The library is one translation unit (lib.cu), so the status word is defined here once.
-__device__ int g_aib_status = 0;
+__device__ int g_aib_status[2] = {0, 0};
 
-AIB_DEV void set_status(int code) { atomicCAS(&g_aib_status, 0, code); }
+AIB_DEV void set_status(int code) { atomicCAS(&g_aib_status[0], 0, code); }
+// What is no failure (a draw beyond the sampler's candidates) has a place of its own, so that it hides none.
+AIB_DEV void set_notice(int code) { atomicCAS(&g_aib_status[1], 0, code); }
 
 // spin limit for bounded waits: 4M tries of a try_wait that suspends up to the hardware's limit -- tens of
 // milliseconds to a few seconds in all, far longer than any legitimate wait in these kernels (the longest is a

@@ -560,9 +560,11 @@ __global__ void __launch_bounds__(Lay<HD>::kThreads, 1)
     int at = batch, iu = beg, is = 0;   // place in the batch of the unit whose copies start next, that unit, its tile
     int started = 0, landed = 0;        // copies of the warp
     const bool withhold = g_aib_withhold_copies != 0;
-// With one tile of query heads a step reads the cache once, so its copies leave L2 first (131072 rows behind other
-    // traffic: 119 -> 107 us). With several, every tile reads the same rows again: they stay as others do (16 sequences of
-    // up to 8192, 16 query heads to a key head of 128, bf16, L2 cold: 82 us, evicted first 92 us; one key head, 32768: 45, 55).
+    // With one tile of query heads a call reads the cache once, so its copies leave L2 first. In a step other data pass between
+    // two visits of a layer's cache; caches in turn, 600 MB of them: 16 sequences of up to 4096 32.2 us, 200 windowed ones 26.8
+    // (without the hint 33.4 and 28.9; a cache that is all in L2 loses, 26.0 and 24.3 us for the windowed one over and over).
+    // With several tiles every one reads the same rows again, and the copies stay as others do: 16 query heads to a key head,
+    // bf16, L2 cold, 16 sequences: 8 key heads, up to 8192 rows 84 us (evicted first 96), one, up to 32768 rows 47 us (55).
     const uint64_t policy = tiles == 1 ? l2_evict_first() : l2_evict_normal();
     // starts the copies of unit iu's K (and returns the unit's attended rows) or V
     auto start = [&](bool v) {

@@ -213,11 +213,13 @@ int aib_debug_knob(int knob, int value) {
 
 int aib_status_read(int* out, int clear) {
   if (!out) return aib::fail(AIB_EINVAL, "aib_status_read: out is NULL");
-  cudaError_t e = cudaMemcpyFromSymbol(out, aib::g_aib_status, sizeof(int));
+  int both[2];
+  cudaError_t e = cudaMemcpyFromSymbol(both, aib::g_aib_status, sizeof(both));
   if (e != cudaSuccess) return aib::fail(AIB_ECUDA, "aib_status_read: %s", cudaGetErrorString(e));
+  *out = both[0] ? both[0] : both[1];
   if (clear) {
-    int z = 0;
-    e = cudaMemcpyToSymbol(aib::g_aib_status, &z, sizeof(int));
+    const int z[2] = {0, 0};
+    e = cudaMemcpyToSymbol(aib::g_aib_status, z, sizeof(z));
     if (e != cudaSuccess) return aib::fail(AIB_ECUDA, "aib_status_read(clear): %s", cudaGetErrorString(e));
   }
   return AIB_OK;

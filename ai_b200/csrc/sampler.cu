@@ -358,7 +358,7 @@ AIB_DEV void sample_row_full(uint8_t* dsm, Shared& sh, const float* __restrict__
   keep = max(1, min(keep, nc));
   // the candidates must contain the nucleus: their total mass reaches top_p, or they are the whole kept set
   if (tid == 0 && nc < sh.ncand_total && (cp[nc - 1] + exp(static_cast<double>(key_value(ckey[nc - 1])) / Td - Mz) / Z) < min(top_p, 1.0 - 1e-12))
-    set_status(AIB_DEV_SAMPLER_CAP);
+    set_notice(AIB_DEV_SAMPLER_CAP);
   const double pl = exp(static_cast<double>(key_value(ckey[keep - 1])) / Td - Mz) / Z;
   const double S = cp[keep - 1] + pl;  // kept mass
   const double u = us ? us[b] : 0.5;

@@ -855,16 +855,21 @@ class PagedBatch(Batch):
 
     def begin(self, adj, rows):
         super().begin(adj, rows)
-        with _lib.on_device(self.eng.device.index):
-            self.clean = _lib.status(clear=False) == 0
+        self.clean = self._failure() == 0
         self.ws.zero_()  # a wait that ran out in an earlier batch may have left counters in it
         for b, n in enumerate(rows):
             self.pages.grow(b, n)
 
-    def check(self):
+    def _failure(self):
         with _lib.on_device(self.eng.device.index):
-            code = _lib.status(clear=self.clean)  # (one of an earlier call stays, and hides what came after it)
-        if code and self.clean:
+            code = _lib.status(clear=False)
+        return 0 if code == _lib.DEV_SAMPLER_CAP else code  # a draw beyond the candidates is a notice
+
+    def check(self):
+        code = self._failure()
+        if code and self.clean:  # (one of an earlier call stays, and hides what came after it)
+            with _lib.on_device(self.eng.device.index):
+                _lib.status(clear=True)
             raise RuntimeError(f"the batch failed on the device: status {code} (AIB_DEV_* in ai_b200.h)")
 
     def end(self):

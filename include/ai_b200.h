@@ -35,7 +35,8 @@ extern "C" {
 #define AIB_ENOTSUP (-4)    /* configuration not supported by this build               */
 #define AIB_ESPACE (-5)     /* output capacity too small (two-pass APIs report need)   */
 
-/* device status codes (aib_status_read) */
+/* device status codes (aib_status_read): the first one recorded stays; AIB_DEV_SAMPLER_CAP,
+ * a notice and no failure, is read where there is no other */
 #define AIB_DEV_TIMEOUT_FULL 101  /* GEMV consumer or paged attention waited too long for a copy */
 #define AIB_DEV_TIMEOUT_EMPTY 102 /* GEMV producer waited too long for a free stage         */
 #define AIB_DEV_BAD_TOKEN 103     /* embedding id outside the vocabulary                     */
@@ -67,7 +68,7 @@ int aib_abi_version(void);
 const char* aib_last_error(void);
 /* Programmatic dependent launch between consecutive kernels (default on). */
 void aib_set_pdl(int enabled);
-/* Device status word of the current device: copies it to *out (synchronous) and, if clear != 0, resets it. */
+/* Device status of the current device: copies it to *out (synchronous) and, if clear != 0, resets it. */
 int aib_status_read(int* out, int clear);
 /* Test knobs of the current device (synchronous; no reference counterpart), so that tests can make a bounded wait
  * run out without any fault: knob 1 = spin limit of every bounded wait (polls; 0 restores the default, 2^22 polls,

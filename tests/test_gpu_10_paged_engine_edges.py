@@ -102,3 +102,32 @@ def test_pages_hold_the_rows_that_are_written_and_no_more(eng):
         if pages > len(lens):
             with pytest.raises(ValueError):
                 eng.generate_batch(prompts, max_new=max_new, page=page, pages=pages - 1)
+
+
+def test_the_samplers_notice_is_no_failure_of_a_batch(eng):
+    """A draw beyond the sampler's candidates (status 105) is noted, not raised, and hides no failure after it."""
+    from ai_b200 import _lib, sampler
+    prompts = prompts_of(eng, (40, 9))
+    want = eng.generate_batch(prompts, max_new=6, page=16)
+    flat = torch.zeros(1, 151936, device="cuda")
+    free = torch.full((1, (eng.V + 31) // 32), -1, dtype=torch.int32)
+
+    def noticed(out):
+        sampler.sample(flat, temperature=1.0, us=[0.999])
+        return free
+
+    assert eng.generate_batch(prompts, max_new=6, page=16, mask=noticed) == want
+    assert _lib.status(clear=False) == 105  # left for whoever asks
+    assert eng.generate_batch(prompts, max_new=6, page=16) == want
+
+    def spoil(out):
+        noticed(out)
+        if len(out[0]) == 2:
+            eng._pbt.pages.table[1, 0] = -5
+        return free
+
+    with pytest.raises(RuntimeError, match="107"):
+        eng.generate_batch(prompts, max_new=5, page=16, mask=spoil)
+    assert _lib.status() == 0
+    sampler.sample(flat, temperature=1.0, us=[0.999])
+    assert _lib.status() == 105
