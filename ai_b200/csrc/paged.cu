@@ -116,9 +116,9 @@ AIB_DEV bool find_seq(const int32_t* cu, const int64_t* pos, int B, int t, int* 
 // with 16-byte accesses and norm and rotation need no exchange but the sum of squares. The norm's weights are folded
 // into the token's cosines and sines, which a warp computes once. The first vectors are on their way before the warp
 // looks for its sequence, position and page, the next ones while it works.
-// Bound by bytes for prompts: 16384 tokens of 32 + 2 x 8 heads of 128 in fp32, 738 MB, 119 us = 6.2 TB/s (two dimensions a
-// lane and norm weights read for every vector: 131 instructions a vector and 135 us). By latency for single tokens: 4.2 us
-// for one, 18 us when one warp did all of its 48 vectors.
+// Bound by bytes for prompts: 16384 tokens of 32 + 2 x 8 heads of 128 in fp32, 738 MB, 118 us = 6.25 TB/s captured (two
+// dimensions a lane and norm weights read for every vector: 131 instructions a vector and 135 us). By latency for single
+// tokens: 2.4 us among captured calls, 4.2 us by itself (18 us when one warp did all of its 48 vectors).
 constexpr int kAppWarps = 8;
 constexpr int kAppSteps = 2;  // steps of 32 / LPV vectors in hand, and as many on their way
 
@@ -284,9 +284,11 @@ __global__ void __launch_bounds__(32 * kAppWarps)
 // rounds, so no long chain runs through one accumulator: the rows' running sums are added outside (131072 rows in fp32:
 // error 3.9e-6 with one accumulator, 3.6e-7 so).
 //
-// Measured (B200, captured): 64 sequences of up to 8192 in bf16, 983 MB, 158 us = 6.2 TB/s; one of 131072 in fp32, 537 MB,
-// 95 us = 5.7 TB/s (a few SMs get 12 % less of the memory and finish last); 16 of up to 4096 33 us, of which about 21 us
-// are the copies, the rest the sum over the lengths, the first look-up and the joins; one of 517 12.6 us, all latency.
+// Measured (B200, captured, caches in turn so that none is left in L2): 64 sequences of up to 8192 in bf16, 983 MB, 157 us =
+// 6.3 TB/s; one of 131072 in fp32, 537 MB, 93 us = 5.8 TB/s (a few SMs get 12 % less of the memory and finish last); 16 of up
+// to 4096 32 us, of which about 21 us are the copies, the rest the sum over the lengths, the first look-up and the joins; 200
+// windowed ones 26 us; one of 517 11 us, all latency. Query heads beyond 8 a key head are another tile, which reads the same
+// rows again (16 sequences of up to 8192, 8 x 16 heads of 128, bf16: 82 us cold, twice its floor of 41).
 // Tried and slower: a copying warp for eight computing ones (single units, 190 us for the 64 sequences: it issued too
 // slowly; batches of look-ups, 157 us, but 36 against 25 us for 200 short ones, whose joins held the warps up), 16-byte
 // asynchronous copies (178 us), runs of two sizes (no change), the joins' code run once ahead of time (+5 us).

@@ -836,9 +836,10 @@ class Adjustment:
 
 
 class PagedBatch(Batch):
-    """A batch whose keys and values lie in pages of one pool [L, 2, pages, KV, page, HD]: a sequence costs the pages that
-    it fills. A prompt runs in the engine's own cache and is then copied to its pages; a step appends every sequence's
-    token to its page and attends over the pages (ai_b200.paged)."""
+    """A batch whose keys and values lie in pages of one pool [L, 2, pages, KV, page, HD]: a sequence costs the pages of its
+    prompt and of the tokens it may get, taken when the batch begins. A prompt runs in the engine's own cache (whose rows
+    are put back) and is then copied to its pages; a step appends every sequence's token to its page and attends over the
+    pages (ai_b200.paged)."""
 
     def __init__(self, eng, B, page, pages):
         self.page, self.n_pages = page, pages
