@@ -92,6 +92,11 @@ bool rows_meet(const Rows2& ra, const Rows2& rb) {
   if (ra.n[0] <= 0 || ra.n[1] <= 0 || rb.n[0] <= 0 || rb.n[1] <= 0) return false;
   Grid2 a = canonical(ra, true), b = canonical(rb, true);
   if (a.last() <= b.base || b.last() <= a.base) return false;
+  // Cuts of one row: what the inner dimensions span lies apart as a whole.
+  if (a.s[0] == b.s[0] || a.n[0] == 1 || b.n[0] == 1) {
+    auto span = [](const Grid2& g) { return g.width + (g.n[1] - 1) * g.s[1]; };
+    if (!lattices_meet(a.base, a.n[0], span(a), b.base, b.n[0], span(b), std::max(a.s[0], b.s[0]))) return false;
+  }
   // the dimension with more rows is looked at as a whole, the other row by row
   auto split = [](const Grid2& g) { return g.n[0] >= g.n[1] ? 0 : 1; };
   const int la = split(a), lb = split(b);

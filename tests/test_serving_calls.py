@@ -1,6 +1,5 @@
 """Calls of the paged cache and the logit adjustment that must be refused before anything is launched, and what the
 wrappers hand on, on tensors that only say that they are on a GPU."""
-import numpy as np
 import pytest
 import torch
 
